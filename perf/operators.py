@@ -235,7 +235,8 @@ def _prepare_attn(case, seed):
     if own:  # a decode step makes this schedule once from its lengths and uses it in every layer
         from mod_b200.ops import native as N
 
-        st["plan"] = N.attn_shared_plan(st["ctx"], st["offs"], st["shared"], cu[-1], H, K, D, cu_q=st["cu"])
+        st["plan"] = N.attn_shared_plan(st["tables"], st["ctx"], st["offs"], st["shared"], cu[-1], H, K, D,
+                                        cu_q=st["cu"])
     return st
 
 
