@@ -134,6 +134,18 @@ void swiglu(const at::Tensor& gu, at::Tensor& out);
 void argmax(const at::Tensor& logits, at::Tensor& out_idx, const c10::optional<at::Tensor>& out_val,
             int64_t index_offset);
 void verify_tokens(const at::Tensor& draft, const at::Tensor& target, at::Tensor& out);
+void attn_shared(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                 const at::Tensor& block_tables, const at::Tensor& ctx_lens, const c10::optional<at::Tensor>& cu_q,
+                 at::Tensor& out, double scale);
+void kv_copy_pages(const std::vector<at::Tensor>& k, const std::vector<at::Tensor>& v, const at::Tensor& src,
+                   const at::Tensor& dst);
+void kv_compact(const std::vector<at::Tensor>& k, const std::vector<at::Tensor>& v, const at::Tensor& tables,
+                const at::Tensor& lens, at::Tensor& out_tables, at::Tensor& remap, at::Tensor& live,
+                at::Tensor& workspace);
+void verify_sampled(const at::Tensor& logits, const at::Tensor& cu, const at::Tensor& drafts,
+                    const at::Tensor& uniforms, const at::Tensor& noise, const at::Tensor& temperature,
+                    const c10::optional<at::Tensor>& draft_probs, at::Tensor& accepted, at::Tensor& token,
+                    at::Tensor& probs);
 }  // namespace mb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -198,5 +210,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu", &mb::swiglu);
   m.def("argmax", &mb::argmax);
   m.def("verify_tokens", &mb::verify_tokens);
+  m.def("attn_shared", &mb::attn_shared);
+  m.def("kv_copy_pages", &mb::kv_copy_pages);
+  m.def("kv_compact", &mb::kv_compact);
+  m.def("verify_sampled", &mb::verify_sampled);
   m.def("read_and_clear_status", &mb::read_and_clear_status);
 }

@@ -212,6 +212,97 @@ def verify_tokens(draft, target, out=None):
     return out
 
 
+class SharedPlan:
+    """Schedule of :func:`attn_shared` for one step's lengths (made by :func:`attn_shared_plan`)."""
+
+    __slots__ = ("tokens", "heads", "kv_heads", "head_dim", "table_shape", "ctx_lens", "group_offs", "shared_lens",
+                 "cu_q")
+
+
+def attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, tokens: int, heads: int, kv_heads: int,
+                     head_dim: int, cu_q=None) -> SharedPlan:
+    """Schedule of :func:`attn_shared` for one step; made once from the step's lengths, used in every layer.
+
+    Sequences [group_offs[g], group_offs[g + 1]) form group g (int32 [G + 1]); their rows of ``block_tables`` agree in
+    the first ``shared_lens[g] // 16`` entries (int32 [G], in tokens), whose pages are then read once for the group.
+    ``ctx_lens`` int32 [B]: tokens of each sequence with its query tokens; 0 for a padded row.  ``cu_q`` int32 [B + 1]:
+    first query token of each sequence; omitted, every sequence has one (``tokens == B``)."""
+    B = block_tables.shape[0]
+    for name, t, n in (("ctx_lens", ctx_lens, B), ("cu_q", cu_q, B + 1)):
+        if t is not None and (t.dtype != torch.int32 or t.numel() != n or t.device != block_tables.device):
+            raise ValueError(f"attn_shared_plan: {name} must be int32 [{n}] on the tables' device")
+    if group_offs.dtype != torch.int32 or shared_lens.dtype != torch.int32 or \
+            group_offs.numel() != shared_lens.numel() + 1:
+        raise ValueError("attn_shared_plan: group_offs must be int32 [G + 1] and shared_lens int32 [G]")
+    if cu_q is None and tokens != B:
+        raise ValueError("attn_shared_plan: without cu_q every sequence has one query token")
+    if head_dim not in (64, 128, 256) or heads % kv_heads:
+        raise ValueError(f"attn_shared_plan: unsupported heads {heads} / {kv_heads} of dim {head_dim}")
+    p = SharedPlan()
+    p.tokens, p.heads, p.kv_heads, p.head_dim = tokens, heads, kv_heads, head_dim
+    p.table_shape = tuple(block_tables.shape)
+    p.ctx_lens, p.group_offs, p.shared_lens, p.cu_q = ctx_lens, group_offs, shared_lens, cu_q
+    return p
+
+
+def attn_shared(q, k_cache, v_cache, block_tables, plan: SharedPlan, out=None, scale: Optional[float] = None):
+    """Attention of a step's query tokens q [T, Hq, D] (D = 64, 128 or 256) over the paged cache, for batches whose
+    sequences come in groups that share a prefix's pages; query i of a sequence's nq sees its first
+    ctx - nq + i + 1 tokens.  Rows that see no token are zero.  ``plan``: from :func:`attn_shared_plan`."""
+    if tuple(q.shape) != (plan.tokens, plan.heads, plan.head_dim) or k_cache.shape[1] != plan.kv_heads or \
+            tuple(block_tables.shape) != plan.table_shape:
+        raise ValueError("attn_shared: the plan was made for other shapes")
+    if out is None:
+        out = torch.empty_like(q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    _C().attn_shared(q, k_cache, v_cache, block_tables, plan.ctx_lens, plan.cu_q, out, scale)
+    return out
+
+
+def kv_copy_pages(k_caches, v_caches, src, dst) -> None:
+    """Page dst[i] becomes a copy of page src[i] in every layer's K and V cache (lists of one tensor a layer, pages
+    first), one launch.  src, dst int32 [n]; a pair with a negative id is skipped.  No page may be the target of two
+    pairs, or a target and a source."""
+    _C().kv_copy_pages(k_caches, v_caches, src, dst)
+
+
+def kv_compact(k_caches, v_caches, tables, lens, out=None):
+    """Moves the live pages (those that ``tables`` int32 [R, max_blocks] refers to within ``lens`` int32 [R] tokens)
+    to the lowest ids in every layer: of n live pages those below n stay, the others take the dead ids below n, in
+    order.  Returns the rewritten tables (entries past a row's length 0), the new id of every page (-1: dead) and
+    n as int32 [1].  ``out`` may be ``tables`` itself."""
+    dev, pages = tables.device, k_caches[0].shape[0]
+    if out is None:
+        out = torch.empty_like(tables)
+    remap = torch.empty(pages, dtype=torch.int32, device=dev)
+    live = torch.empty(1, dtype=torch.int32, device=dev)
+    ws = torch.empty(3 * pages + 1, dtype=torch.int32, device=dev)
+    _C().kv_compact(k_caches, v_caches, tables, lens, out, remap, live, ws)
+    return out, remap, live
+
+
+def verify_sampled(logits, cu, drafts, uniforms, noise, temperature, draft_probs=None):
+    """Accepts or refuses drafted tokens so that what is emitted follows the target's distribution.
+
+    logits [rows, V] bf16 or fp32: rows cu[b] .. cu[b + 1] - 1 are sequence b's, one for each of its drafts and one
+    more (cu int32 [B + 1]); drafts int64 [B, K]; uniforms fp32 [B, K] in [0, 1); noise fp32 [B, V] ~ Exp(1);
+    temperature fp32 [B] (<= 0: greedy); draft_probs [B, K, V] fp32 or bf16: the distributions that the drafts were
+    drawn from (omitted: the drafts were certain, as n-gram drafts are).
+
+    With p = softmax(logits / temperature), draft d is accepted where u q(d) < p(d).  At the first refusal the next
+    token is argmax of (p - q)+ / noise, after the last acceptance argmax of p / noise.  Returns the number of
+    accepted drafts int32 [B], the next token int64 [B] (-1 where a row has no finite logit) and p of each emitted
+    token fp32 [B, K + 1] (0 past the next token)."""
+    B, K = drafts.shape
+    dev = logits.device
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    token = torch.empty(B, dtype=torch.int64, device=dev)
+    probs = torch.empty(B, K + 1, dtype=torch.float32, device=dev)
+    _C().verify_sampled(logits, cu, drafts, uniforms, noise, temperature, draft_probs, accepted, token, probs)
+    return accepted, token, probs
+
+
 def deltanet_decode(mixed, z, ba, conv_w, conv_state, ssm, slots, A_log, dt_bias, norm_w, Hk: int, Hv: int,
                     dk: int, dv: int, eps: float, out=None):
     """Fused gated-DeltaNet decode step (conv, L2 norms, gates, delta rule, gated RMSNorm).

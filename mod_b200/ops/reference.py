@@ -216,3 +216,97 @@ def verify_tokens(draft, target, out=None):
         out.copy_(r)
         return out
     return r
+
+
+def attn_shared(q, k_cache, v_cache, block_tables, ctx_lens, cu_q=None, scale=None):
+    """Attention of each sequence's query tokens over its own table; sharing changes what is read, not the result."""
+    T, Hq, D = q.shape
+    Hkv = k_cache.shape[1]
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    cu = list(range(T + 1)) if cu_q is None else cu_q.tolist()
+    res = torch.zeros_like(q)
+    for b, n in enumerate(ctx_lens.tolist()):
+        t0, t1 = cu[b], cu[b + 1]
+        if n <= 0 or t0 == t1:
+            continue
+        k = gather_kv(k_cache, block_tables[b], n).float()    # [n, Hkv, D]
+        v = gather_v(v_cache, block_tables[b], n).float()
+        qb = q[t0:t1].float().view(t1 - t0, Hkv, Hq // Hkv, D)
+        s = torch.einsum("qhgd,nhd->qhgn", qb, k) * scale
+        seen = torch.arange(n, device=q.device)[None, :] <= n - (t1 - t0) + torch.arange(t1 - t0, device=q.device)[:, None]
+        p = torch.softmax(s.masked_fill(~seen[:, None, None, :], float("-inf")), dim=-1)
+        o = torch.where(seen.any(-1)[:, None, None, None], torch.einsum("qhgn,nhd->qhgd", p, v), 0.0)
+        res[t0:t1] = o.reshape(t1 - t0, Hq, D).to(q.dtype)
+    return res
+
+
+def kv_copy_pages(k_caches, v_caches, src, dst):
+    ok = (src >= 0) & (dst >= 0)
+    s, d = src[ok].long(), dst[ok].long()
+    for c in (*k_caches, *v_caches):
+        c[d] = c[s]
+
+
+def kv_compact(k_caches, v_caches, tables, lens):
+    pages = k_caches[0].shape[0]
+    used = torch.arange(tables.shape[1], device=tables.device)[None, :] < ((lens + 15) // 16)[:, None]
+    mark = torch.zeros(pages, dtype=torch.bool, device=tables.device)
+    mark[tables[used].long()] = True
+    n, ids = int(mark.sum()), torch.arange(pages, device=tables.device)
+    src, dst = (mark & (ids >= n)).nonzero().flatten(), (~mark & (ids < n)).nonzero().flatten()
+    remap = torch.where(mark, ids, -1)
+    remap[src] = dst
+    for c in (*k_caches, *v_caches):
+        c[dst] = c[src]
+    out = torch.where(used, remap[tables.long().clamp(0, pages - 1)], 0)
+    return out.int(), remap.int(), torch.tensor([n], dtype=torch.int32, device=tables.device)
+
+
+def verify_sampled(logits, cu, drafts, uniforms, noise, temperature, draft_probs=None):
+    """One sequence and one draft after another; see ``native.verify_sampled``."""
+    B, K = drafts.shape
+    V = logits.shape[1]
+    accepted = torch.zeros(B, dtype=torch.int32)
+    token = torch.full((B,), -1, dtype=torch.int64)
+    probs = torch.zeros(B, K + 1)
+
+    def target(row, t):
+        x = logits[row].float()
+        x = torch.where(torch.isnan(x), float("-inf"), x)
+        top = x.max()
+        if top == float("-inf"):
+            return torch.zeros_like(x)
+        if not t > 0:
+            return torch.zeros_like(x).index_fill_(0, x.argmax(), 1.0)
+        e = torch.where(x == top, 1.0, torch.exp((x - top) / t))
+        return e / e.sum()
+
+    offs, heat, us, ds = cu.tolist(), temperature.tolist(), uniforms.cpu(), drafts.tolist()
+    for b in range(B):
+        n, a = offs[b + 1] - offs[b] - 1, 0
+        while True:
+            p = target(offs[b] + a, heat[b])
+            rest = p
+            if a < n:
+                d = ds[b][a]
+                inside = 0 <= d < V
+                if draft_probs is not None:
+                    q = draft_probs[b, a].float()
+                else:
+                    q = torch.zeros_like(p)
+                    if inside:
+                        q[d] = 1.0
+                if inside and float(us[b, a]) * float(q[d]) < float(p[d]):
+                    probs[b, a] = p[d]
+                    a += 1
+                    continue
+                rest = (p - q).clamp(min=0.0)
+                rest = rest if bool((rest > 0).any()) else p
+            accepted[b] = a
+            if bool((rest > 0).any()):
+                v = int(torch.where(rest > 0, rest / noise[b], -1.0).argmax())
+                token[b], probs[b, a] = v, p[v]
+            break
+    dev = logits.device
+    return accepted.to(dev), token.to(dev), probs.to(dev)
