@@ -134,8 +134,13 @@ void swiglu(const at::Tensor& gu, at::Tensor& out);
 void argmax(const at::Tensor& logits, at::Tensor& out_idx, const c10::optional<at::Tensor>& out_val,
             int64_t index_offset);
 void verify_tokens(const at::Tensor& draft, const at::Tensor& target, at::Tensor& out);
+std::tuple<int64_t, int64_t> attn_shared_sizes(int64_t T, int64_t B, int64_t G, int64_t Hq, int64_t Hkv, int64_t D,
+                                               int64_t max_blocks, int64_t device);
+void attn_shared_plan(const at::Tensor& block_tables, const at::Tensor& ctx_lens, const at::Tensor& group_offs,
+                      const at::Tensor& shared_lens, const c10::optional<at::Tensor>& cu_q, int64_t T, int64_t Hq,
+                      int64_t Hkv, int64_t D, at::Tensor& plan);
 void attn_shared(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
-                 const at::Tensor& block_tables, const at::Tensor& ctx_lens, const c10::optional<at::Tensor>& cu_q,
+                 const at::Tensor& block_tables, int64_t groups, at::Tensor& plan, at::Tensor& workspace,
                  at::Tensor& out, double scale);
 void kv_copy_pages(const std::vector<at::Tensor>& k, const std::vector<at::Tensor>& v, const at::Tensor& src,
                    const at::Tensor& dst);
@@ -210,6 +215,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu", &mb::swiglu);
   m.def("argmax", &mb::argmax);
   m.def("verify_tokens", &mb::verify_tokens);
+  m.def("attn_shared_sizes", &mb::attn_shared_sizes);
+  m.def("attn_shared_plan", &mb::attn_shared_plan);
   m.def("attn_shared", &mb::attn_shared);
   m.def("kv_copy_pages", &mb::kv_copy_pages);
   m.def("kv_compact", &mb::kv_compact);

@@ -215,33 +215,30 @@ def verify_tokens(draft, target, out=None):
 class SharedPlan:
     """Schedule of :func:`attn_shared` for one step's lengths (made by :func:`attn_shared_plan`)."""
 
-    __slots__ = ("tokens", "heads", "kv_heads", "head_dim", "table_shape", "ctx_lens", "group_offs", "shared_lens",
-                 "cu_q")
+    __slots__ = ("tokens", "heads", "kv_heads", "head_dim", "table_shape", "groups", "buf", "ws_elems")
 
 
 def attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, tokens: int, heads: int, kv_heads: int,
-                     head_dim: int, cu_q=None) -> SharedPlan:
+                     head_dim: int, cu_q=None, plan: Optional[SharedPlan] = None) -> SharedPlan:
     """Schedule of :func:`attn_shared` for one step; made once from the step's lengths, used in every layer.
 
     Sequences [group_offs[g], group_offs[g + 1]) form group g (int32 [G + 1]); their rows of ``block_tables`` agree in
     the first ``shared_lens[g] // 16`` entries (int32 [G], in tokens), whose pages are then read once for the group.
     ``ctx_lens`` int32 [B]: tokens of each sequence with its query tokens; 0 for a padded row.  ``cu_q`` int32 [B + 1]:
-    first query token of each sequence; omitted, every sequence has one (``tokens == B``)."""
-    B = block_tables.shape[0]
-    for name, t, n in (("ctx_lens", ctx_lens, B), ("cu_q", cu_q, B + 1)):
-        if t is not None and (t.dtype != torch.int32 or t.numel() != n or t.device != block_tables.device):
-            raise ValueError(f"attn_shared_plan: {name} must be int32 [{n}] on the tables' device")
-    if group_offs.dtype != torch.int32 or shared_lens.dtype != torch.int32 or \
-            group_offs.numel() != shared_lens.numel() + 1:
-        raise ValueError("attn_shared_plan: group_offs must be int32 [G + 1] and shared_lens int32 [G]")
-    if cu_q is None and tokens != B:
-        raise ValueError("attn_shared_plan: without cu_q every sequence has one query token")
-    if head_dim not in (64, 128, 256) or heads % kv_heads:
-        raise ValueError(f"attn_shared_plan: unsupported heads {heads} / {kv_heads} of dim {head_dim}")
-    p = SharedPlan()
+    first query token of each sequence; omitted, every sequence has one (``tokens == B``).
+
+    The schedule is made on the device from the lengths' values at that time (one launch, no synchronisation, capturable
+    in a CUDA graph).  ``plan``: an earlier one of the same sizes, whose buffer is used again."""
+    B, G = block_tables.shape[0], shared_lens.numel()
+    n, ws = _C().attn_shared_sizes(tokens, B, G, heads, kv_heads, head_dim, block_tables.shape[1],
+                                   block_tables.device.index or 0)
+    p = SharedPlan() if plan is None else plan
+    if plan is None:
+        p.buf = torch.empty(n, dtype=torch.int32, device=block_tables.device)
     p.tokens, p.heads, p.kv_heads, p.head_dim = tokens, heads, kv_heads, head_dim
-    p.table_shape = tuple(block_tables.shape)
-    p.ctx_lens, p.group_offs, p.shared_lens, p.cu_q = ctx_lens, group_offs, shared_lens, cu_q
+    p.table_shape, p.groups, p.ws_elems = tuple(block_tables.shape), G, ws
+    _C().attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, cu_q, tokens, heads, kv_heads, head_dim,
+                          p.buf)
     return p
 
 
@@ -256,7 +253,8 @@ def attn_shared(q, k_cache, v_cache, block_tables, plan: SharedPlan, out=None, s
         out = torch.empty_like(q)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    _C().attn_shared(q, k_cache, v_cache, block_tables, plan.ctx_lens, plan.cu_q, out, scale)
+    ws = torch.empty(plan.ws_elems, dtype=torch.float32, device=q.device)
+    _C().attn_shared(q, k_cache, v_cache, block_tables, plan.groups, plan.buf, ws, out, scale)
     return out
 
 
