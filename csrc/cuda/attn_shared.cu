@@ -19,14 +19,15 @@
 // prefix and a tail, leave (o, m, l) partials in fp32 which the merge kernel joins; the others are written at once.
 //
 // The attention kernel is one persistent CTA per SM:
-//   TMA warp   : key tiles (K, then V) of 128 tokens (64 at D = 256), one copy per page, into a ring of 32 KB slots
-//   Q warp     : the rows of the next pieces into two tile buffers (128-byte swizzle, cp.async)
+//   TMA warp   : key tiles (K, then V) of 64 tokens, one copy per page, into a ring of slots
+//   Q warp     : the rows of the next pieces into two tile buffers (128-byte swizzle; by cp.async where the heads of a
+//                group do not divide a tile)
 //   MMA warp   : S = Q.K^T (fp32 in TMEM), O += P.V with P read from TMEM (it overwrites S
 //                as bf16; 32 columns of S hold 32 keys' P and, where it has two terms, the second one's)
 //   2 x 8 warps: softmax of one 128-row tile each, a row a thread; a row's O is rescaled only where its running
 //                maximum has grown by more than 2^8 (P stays below 256, so bf16 and fp32 lose nothing)
-// The two tiles are independent pipelines that share the tensor cores: while one's softmax runs, the other's products
-// do.  A piece of one tile only lets its even and odd key tiles take the two pipelines and joins their halves in TMEM.
+// The two tiles are independent pipelines that share the tensor cores, and each has two S: while the softmax of one
+// runs, the products of the other are done.  A piece of one tile only lets its even and odd key tiles take the two pipelines and joins their halves in TMEM.
 // At D = 256 TMEM holds one pipeline.  Sums, maxima and O stay in fp32.  For one-tile pieces, which wait for memory and
 // not for the tensor cores, P enters the second product as two bf16 terms (16 bits of it, over S's whole columns), so
 // that few keys leave no more than the output's rounding; two-tile pieces round P to bf16, whose errors of 2^-9 average
@@ -50,14 +51,14 @@ namespace {
 
 constexpr int kWideRows = 256;    // rows of a prefix unit at D <= 128 (two tiles)
 constexpr int kTileRows = 128;
+constexpr int kTileKeys = 64;
 constexpr int kNoLimit = 1 << 29;
 constexpr int kLeanRows = 64;     // sequences of up to this many rows take the lean kernel for their own tokens (D <= 128)
 constexpr int kLeanWarps = 16;    // lean pieces aimed at, for each SM
 constexpr int kSplitKeys = 4096;  // prefixes below this enter the second product as two bf16 terms as well
 
-// Costs of a unit in the units of one 128-key tile of one row tile: a wide tile does the products of two, a unit
-// costs its start and its end besides.
-constexpr int kCostNarrow = 2, kCostWide = 3, kCostUnit = 2;
+// Costs: a tile of keys against one and against two tiles of rows, and a unit's start and end.
+constexpr int kCostNarrow = 2, kCostWide = 3, kCostUnit = 8;
 
 struct Unit {
   int row0;      // first row, in (token, head of the group) order
@@ -93,7 +94,7 @@ struct PlanView {
 };
 
 struct PlanDims {
-  int T, B, G, Gq, Hkv, tile_keys, wide_rows, shares, max_blocks, max_units, max_pieces, lean_rows;
+  int T, B, G, Gq, Hkv, wide_rows, shares, max_blocks, max_units, max_pieces, lean_rows;
 };
 
 __host__ __device__ inline int64_t plan_ints(const PlanDims& d) {
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(kPlanThreads)
       u.key_end = min(ctx_of(b), u.lim + (u.row0 + u.rows - 1) / d.Gq);
       u.solo = u.key0 == 0;
     }
-    u.tiles = max(0, (u.key_end - u.key0 + d.tile_keys - 1) / d.tile_keys);
+    u.tiles = max(0, (u.key_end - u.key0 + kTileKeys - 1) / kTileKeys);
     reinterpret_cast<Unit*>(v.units)[i] = u;
     v.cost[i] = u.tiles * (u.rows > kTileRows ? kCostWide : kCostNarrow) + kCostUnit;
     v.rowcum[i] = u.rows;
@@ -334,17 +335,17 @@ __global__ void __launch_bounds__(kPlanThreads)
 template <int D>
 struct Cfg {
   static constexpr int kPipes = D > 128 ? 1 : 2;
-  static constexpr int kKeys = D > 128 ? 64 : 128;      // keys of a tile
+  static constexpr int kKeys = kTileKeys;
   static constexpr int kBlocks = kKeys / 16;
   static constexpr int kChunks = D / 64;
   static constexpr int kSlot = kKeys * D * 2;           // K or V of a tile
-  static constexpr int kSlots = D == 64 ? 8 : 5;
+  static constexpr int kSlots = D > 128 ? 5 : 10;
   static constexpr int kQBytes = kTileRows * D * 2;
   static constexpr int kSoftWarps = kPipes * 4;
-  static constexpr int kThreads = kSoftWarps * 32 + 96;
+  static constexpr int kThreads = (kSoftWarps + kPipes + 2) * 32;
   static constexpr int kSmem = 1024 + kPipes * kQBytes + kSlots * kSlot + kTileRows * 8 + 256;
-  // TMEM: S (and P over it) of each pipeline in its own 128 columns, O behind them
-  static __device__ __forceinline__ uint32_t s_col(int p) { return p * 128; }
+  // TMEM: two S (and P over them) of each pipeline, O behind them
+  static __device__ __forceinline__ uint32_t s_col(int p, int i) { return p * 128 + i * kKeys; }
   static __device__ __forceinline__ uint32_t o_col(int p) { return 256 + p * D; }
 };
 
@@ -441,6 +442,12 @@ __device__ __forceinline__ float2 add2(float2 x, float2 y) {
       : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
   return r;
 }
+// A whole 32-byte sector: lanes write rows of their own, and half sectors would be written twice.
+__device__ __forceinline__ void store32(float* p, const float* f) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]),
+               "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+               : "memory");
+}
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(~0u, x, 0); }
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -494,6 +501,7 @@ struct AttnArgs {
   float2* part_ml; // [partial rows] (maximum, sum)
   int* plan;
   PlanDims dims;
+  int tma_q;       // a 128-row tile is a number of whole tokens
   int Hq, pages, over;  // over: first partial row of pieces that begin inside a unit (256 for each share)
   float scale_log2;
   int* status;
@@ -501,8 +509,8 @@ struct AttnArgs {
 
 template <int D>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
-    attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                       const __grid_constant__ AttnArgs a) {
+    attn_shared_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a) {
   using C = Cfg<D>;
   constexpr int NP = C::kPipes, KT = C::kKeys, NS = C::kSlots;
   extern __shared__ uint8_t smem_raw[];
@@ -515,9 +523,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   uint64_t* empty = full + NS;       // [NS]
   uint64_t* q_full = empty + NS;     // [NP]
   uint64_t* q_empty = q_full + NP;   // [NP]
-  uint64_t* s_ready = q_empty + NP;  // [NP] scores are in TMEM
-  uint64_t* p_ready = s_ready + NP;  // [NP] weights are in TMEM, O may be accumulated
-  uint64_t* o_done = p_ready + NP;   // [NP] a piece's last product is complete
+  uint64_t* s_ready = q_empty + NP;  // [NP][2] scores are in TMEM
+  uint64_t* p_ready = s_ready + 2 * NP;  // [NP][2] weights are in TMEM, O may be accumulated
+  uint64_t* pv_done = p_ready + 2 * NP;  // [NP] a tile's second product is complete
+  uint64_t* o_done = pv_done + NP;   // [NP] a piece's last one is
   uint64_t* o_free = o_done + NP;    // [NP] O has been read
   uint64_t* stat_ready = o_free + NP;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stat_ready + 1);
@@ -526,13 +535,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], NP);
     }
     for (int i = 0; i < NP; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
-      mbar_init(&s_ready[i], 1);
-      mbar_init(&p_ready[i], 4);
+      mbar_init(&q_empty[i], NP);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&s_ready[2 * i + k], 1);
+        mbar_init(&p_ready[2 * i + k], 4);
+      }
+      mbar_init(&pv_done[i], 1);
       mbar_init(&o_done[i], 1);
       mbar_init(&o_free[i], 4);
     }
@@ -543,7 +555,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (tid == C::kSoftWarps * 32 + 32) {
+  if (tid == (C::kSoftWarps + NP) * 32) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
@@ -558,31 +570,36 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   const PlanView pv = plan_view(a.plan, a.dims);
   Walk w(pv, blockIdx.x);
 
-  if (warp == C::kSoftWarps) {
+  if (warp >= C::kSoftWarps && warp < C::kSoftWarps + NP) {
     // ---------------------------------------------------------------- MMA
-    // The whole warp walks and waits, one elected lane issues, and what an instruction takes is made uniform first: a
-    // product that one lane of a divergent warp issues costs over 200 clocks, three times its 64 on the tensor cores.
+    // A warp for each pipeline.  The whole warp walks and waits, one elected lane issues, and what an instruction takes
+    // is made uniform first: a product that one lane of a divergent warp issues costs over 200 clocks, three times its
+    // 64 on the tensor cores.
     constexpr uint32_t idesc_s = make_idesc_bf16(128, KT), idesc_o = make_idesc_bf16(128, D);
     const bool el = elect_one_sync();
+    const int p = (int)uniform(warp - C::kSoftWarps);
     const uint32_t tm = uniform(tmem);
-    struct Pipe {  // scores whose second product has not been issued, and counts
-      uint32_t slot, par, visits, pieces;
+    struct Pending {  // scores whose second product has not been issued
+      uint32_t slot, par;
       int blocks;
-      bool any, first, last, free_v, split;
-    } p0 = {}, p1 = {};
+      bool any, first, last;
+    } pend0 = {}, pend1 = {};
+    uint32_t visits = 0, begun = 0, starts = 0;  // first products, second products, pieces
     uint32_t q_par = 0, tile = 0, n = 0, qn = 0;
     bool ok = true;
-    auto finish = [&](Pipe& x, const int p) {  // O += P.V
+    auto finish = [&](Pending& x, const int i) {  // O += P.V of scores i
       if (!x.any || !ok) return;
       x.any = false;
-      ok = bar_wait(&p_ready[p], (x.visits - 1) & 1, a.status) && bar_wait(&full[x.slot], x.par, a.status);
-      if (x.first && x.pieces > 1) ok = ok && bar_wait(&o_free[p], x.pieces & 1, a.status);
+      ok = bar_wait(&p_ready[2 * p + i], (begun >> 1) & 1, a.status) && bar_wait(&full[x.slot], x.par, a.status);
+      ++begun;
+      starts += x.first;
+      if (x.first && starts > 1) ok = ok && bar_wait(&o_free[p], starts & 1, a.status);
       ok = __all_sync(~0u, ok);
       if (!ok) return;
       tc_fence_after();
       const uint32_t slot = uniform(x.slot);
       const uint64_t vd = desc_k32(smem_u32(sKV) + slot * C::kSlot);
-      const uint32_t o = tm + C::o_col(p), w0 = tm + C::s_col(p);
+      const uint32_t o = tm + C::o_col(p), w0 = tm + C::s_col(p, i);
       const uint32_t acc = uniform(!x.first);
       const int blocks = (int)uniform(x.blocks);
       if (el) {
@@ -590,7 +607,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 #pragma unroll
           for (int kb = 0; kb < C::kBlocks; ++kb)
             mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8, vd + kb * (D * 32 / 16), idesc_o, kb ? 1 : acc);
-          if (x.split) {
+          if (w.split) {
 #pragma unroll
             for (int kb = 0; kb < C::kBlocks; ++kb)
               mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8 + 16, vd + kb * (D * 32 / 16), idesc_o, 1);
@@ -599,19 +616,22 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 #pragma unroll 1
           for (int kb = 0; kb < blocks; ++kb) {
             mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8, vd + kb * (D * 32 / 16), idesc_o, kb ? 1 : acc);
-            if (x.split) mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8 + 16, vd + kb * (D * 32 / 16), idesc_o, 1);
+            if (w.split) mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8 + 16, vd + kb * (D * 32 / 16), idesc_o, 1);
           }
         }
-        if (x.free_v) tc_commit(&empty[slot]);
+        tc_commit(&empty[slot]);
+        tc_commit(&pv_done[p]);
         if (x.last) tc_commit(&o_done[p]);
       }
       __syncwarp();
     };
-    // one tile's products on pipeline p: the second one of its last scores, the first one of these
-    auto event = [&](Pipe& x, const int p, int j, int nt, int blocks, uint32_t buf_, bool last_event) {
-      finish(x, p);
-      const uint32_t buf = uniform(buf_), kslot = uniform((2 * tile) % NS);
-      if (j == 0) ok = __all_sync(~0u, ok && bar_wait(&q_full[buf], (q_par >> buf) & 1, a.status));
+    // S = Q.K^T of a tile into scores i, after the second product of what was there
+    auto begin = [&](Pending& x, const int i, uint32_t load, uint32_t buf, int blocks, bool first, bool last) {
+      finish(x, i);
+      const uint32_t kslot = uniform(load % NS);
+      ok = ok && bar_wait(&full[kslot], (load / NS) & 1, a.status);
+      if (first) ok = ok && bar_wait(&q_full[buf], (q_par >> buf) & 1, a.status);
+      ok = __all_sync(~0u, ok);
       if (!ok) return;
       tc_fence_after();
       const uint64_t qd = desc_k128(smem_u32(sQ) + buf * C::kQBytes, 1024);
@@ -619,52 +639,61 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       if (el) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          tc_mma_bf16(tm + C::s_col(p), qd + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16,
+          tc_mma_bf16(tm + C::s_col(p, i), qd + ((kk >> 2) * 16384 + (kk & 3) * 32) / 16,
                       kd + ((kk >> 2) * 1024 + (kk & 3) * 32) / 16, idesc_s, kk > 0);
-        tc_commit(&s_ready[p]);
-        if (last_event) tc_commit(&empty[kslot]);
-        if (j == nt - 1) tc_commit(&q_empty[buf]);
+        tc_commit(&s_ready[2 * p + i]);
+        tc_commit(&empty[kslot]);
       }
       __syncwarp();
-      if (j == nt - 1) q_par ^= 1u << buf;
-      x.slot = (2 * tile + 1) % NS;
-      x.par = ((2 * tile + 1) / NS) & 1;
+      x.slot = (load + 1) % NS;
+      x.par = ((load + 1) / NS) & 1;
       x.blocks = blocks;
       x.any = true;
-      x.first = w.wide ? j == 0 : j < NP;
-      x.last = w.wide ? j == nt - 1 : j >= nt - NP;
-      x.free_v = last_event;
-      x.split = w.split;
-      ++x.visits;
-      x.pieces += x.first;
+      x.first = first;
+      x.last = last;
+      ++visits;
     };
     while (ok && w.next()) {
-      const int nt = w.t1 - w.t0;
+      const int nt = w.t1 - w.t0, step = w.wide ? 1 : NP, bufs = w.wide ? NP : 1;
+      const int j0 = w.wide ? 0 : (int)((p + NP - n % NP) % NP);  // this pipeline's first tile
       const int keys = w.e.key_end - w.e.key0 - w.t0 * KT;
+      const uint32_t buf = uniform((qn + (w.wide ? p : 0)) % NP);
       for (int j = 0; j < nt && ok; ++j, ++tile) {
-        const int blocks = (min(KT, keys - j * KT) + 15) / 16;
-        ok = __all_sync(~0u, bar_wait(&full[(2 * tile) % NS], ((2 * tile) / NS) & 1, a.status));
-        if (w.wide) {
-          event(p0, 0, j, nt, blocks, qn % NP, NP == 1);
-          if (NP == 2) event(p1, 1, j, nt, blocks, (qn + 1) % NP, true);
-        } else if (NP == 1 || n % 2 == 0) {
-          event(p0, 0, j, nt, blocks, qn % NP, true);
-        } else {
-          event(p1, 1, j, nt, blocks, qn % NP, true);
+        const uint32_t load = 2 * tile;
+        if (j >= j0 && (j - j0) % step == 0) {
+          const int blocks = (min(KT, keys - j * KT) + 15) / 16;
+          const bool first = j == j0, last = j + step >= nt;
+          if (visits & 1) begin(pend1, 1, load, buf, blocks, first, last);
+          else begin(pend0, 0, load, buf, blocks, first, last);
+        } else {  // the other pipeline's: seen to have arrived, and given up
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const uint32_t slot = (load + kv) % NS;
+            ok = ok && bar_wait(&full[slot], ((load + kv) / NS) & 1, a.status);
+            if (ok && el) mbar_arrive(&empty[slot]);
+          }
+          ok = __all_sync(~0u, ok);
         }
-        ++n;
       }
-      qn += w.wide ? NP : 1;
-      if (w.wide) n = 0;  // the first pipeline goes on: the second one's product frees the tile that both read
+      // the rows are free when both pipelines are done with them
+      for (int i = 0; i < bufs; ++i) {
+        const uint32_t b = (qn + i) % NP;
+        ok = __all_sync(~0u, ok && bar_wait(&q_full[b], (q_par >> b) & 1, a.status));
+        if (ok && el) tc_commit(&q_empty[b]);
+        q_par ^= 1u << b;
+      }
+      // a piece's last second products wait for no later piece: their results may free what that one waits for
+      if (visits & 1) {
+        finish(pend1, 1);
+        finish(pend0, 0);
+      } else {
+        finish(pend0, 0);
+        finish(pend1, 1);
+      }
+      qn += bufs;
+      n = w.wide ? 0 : n + nt;
     }
-    if (NP == 2 && n % 2 == 1) {
-      finish(p1, NP - 1);
-      finish(p0, 0);
-    } else {
-      finish(p0, 0);
-      if (NP == 2) finish(p1, NP - 1);
-    }
-  } else if (warp == C::kSoftWarps + 1) {
+  } else if (warp == C::kSoftWarps + NP) {
     // ---------------------------------------------------------------- K and V loads
     const bool el = elect_one_sync();
     uint32_t load = 0;
@@ -711,21 +740,32 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     // no copy may be in flight when the CTA leaves
     if (lane == 0)
       for (uint32_t i = load > NS ? load - NS : 0; i < load; ++i) bar_wait(&full[i % NS], (i / NS) & 1, a.status);
-  } else if (warp == C::kSoftWarps + 2) {
+  } else if (warp == C::kSoftWarps + NP + 1) {
     // ---------------------------------------------------------------- Q rows
-    uint32_t uses[NP], qn = 0;
-    for (int p = 0; p < NP; ++p) uses[p] = 0;
+    const bool el = elect_one_sync();
+    uint32_t uses = 0, qn = 0;  // uses: a bit for each buffer
     bool ok = true;
     constexpr int kLanes = D / 8;  // 16-byte pieces of a row
     while (ok && w.next()) {
       for (int i = 0; i < (w.wide ? NP : 1); ++i, ++qn) {
         const int buf = qn % NP;
-        if (lane == 0) ok = bar_wait(&q_empty[buf], (uses[buf] & 1) ^ 1, a.status);
+        if (lane == 0) ok = bar_wait(&q_empty[buf], ((uses >> buf) & 1) ^ 1, a.status);
         ok = __shfl_sync(~0u, ok, 0);
         if (!ok) break;
-        ++uses[buf];
+        uses ^= 1u << buf;
         const int rows = min(kTileRows, w.e.rows - i * kTileRows);
         const int row0 = w.e.row0 + i * kTileRows;
+        if (a.tma_q) {  // whole tokens: rows past the unit's are other tokens' and are ignored
+          const uint32_t ub = uniform(buf), token = uniform(row0 / a.dims.Gq), head = uniform(w.hk * a.dims.Gq);
+          if (el) {
+            mbar_arrive_expect_tx(&q_full[ub], C::kQBytes);
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_load_3d(sQ + ub * C::kQBytes + c * 16384, &tmQ, &q_full[ub], c * 64, head, token);
+          }
+          __syncwarp();
+          continue;
+        }
 #pragma unroll 4
         for (int x = lane; x < rows * kLanes; x += 32) {
           const int r = x / kLanes, c = x % kLanes, tok = (row0 + r) / a.dims.Gq, g = (row0 + r) % a.dims.Gq;
@@ -744,7 +784,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     // ---------------------------------------------------------------- softmax, a row a thread
     const int p = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes + C::s_col(p), tO = tmem + lanes + C::o_col(p);
+    const uint32_t tO = tmem + lanes + C::o_col(p);
     uint32_t n = 0, tile = 0, visits = 0, pieces0 = 0, pieces1 = 0, joins = 0;
     bool ok = true;
     while (ok && w.next()) {
@@ -760,7 +800,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       const int j0 = wide ? 0 : (int)((p + NP - n % NP) % NP);  // this pipeline's first tile
       const bool mine = j0 < nt;
       for (int j = j0; j < nt; j += wide ? 1 : NP) {
-        if (lane == 0) ok = bar_wait(&s_ready[p], visits & 1, a.status);
+        const int at = 2 * p + (visits & 1);
+        const uint32_t tS = tmem + lanes + C::s_col(p, visits & 1);
+        if (lane == 0) ok = bar_wait(&s_ready[at], (visits >> 1) & 1, a.status);
         ok = __shfl_sync(~0u, ok, 0);
         ++visits;
         if (!ok) break;
@@ -784,6 +826,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
           if (j == j0) {
             m = mx;
           } else if (__any_sync(~0u, row < rows && mx > m + 8.f)) {
+            // (O is complete up to the tile before: its second product has been)
+            if (lane == 0) ok = bar_wait(&pv_done[p], (visits - 2) & 1, a.status);
+            ok = __shfl_sync(~0u, ok, 0);
+            if (!ok) break;
+            tc_fence_after();
             const bool up = row < rows && mx > m + 8.f;
             const float f = up ? ex2(m - mx) : 1.f;  // rows that stay are multiplied by one: bit for bit as they were
             if (up) m = mx;
@@ -842,7 +889,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[p]);
+        if (lane == 0) mbar_arrive(&p_ready[at]);
       }
       if (!ok) break;
       // ---- the piece's result
@@ -911,9 +958,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
                     make_uint4(pack_bf16(f[e], f[e + 1]), pack_bf16(f[e + 2], f[e + 3]),
                                pack_bf16(f[e + 4], f[e + 5]), pack_bf16(f[e + 6], f[e + 7]));
             } else if (valid) {
-#pragma unroll
-              for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<float4*>(part + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+              store32(part + c, f);
+              store32(part + c + 8, f + 8);
             }
           }
         }
@@ -1228,7 +1274,6 @@ PlanDims plan_dims(int64_t T, int64_t B, int64_t G, int64_t Hq, int64_t Hkv, int
                    int device) {
   PlanDims d;
   d.T = (int)T, d.B = (int)B, d.G = (int)G, d.Gq = (int)(Hq / Hkv), d.Hkv = (int)Hkv;
-  d.tile_keys = D > 128 ? 64 : 128;
   d.wide_rows = D > 128 ? kTileRows : kWideRows;
   d.shares = sm_count(device);
   d.max_blocks = (int)max_blocks;
@@ -1307,7 +1352,7 @@ void attn_shared_plan(const at::Tensor& block_tables, const at::Tensor& ctx_lens
 }
 
 template <int D>
-static void launch_attn(const at::Tensor& k_cache, const at::Tensor& v_cache, AttnArgs a, cudaStream_t st, int dev) {
+static void launch_attn(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, AttnArgs a, cudaStream_t st, int dev) {
   using C = Cfg<D>;
   const cuuint64_t heads = (cuuint64_t)k_cache.size(0) * k_cache.size(1);
   // K as (64 elements, 8 rows, D / 64 chunks, groups of 8 rows): a page's two groups arrive as swizzle atoms
@@ -1315,6 +1360,10 @@ static void launch_attn(const at::Tensor& k_cache, const at::Tensor& v_cache, At
   const cuuint32_t kb[4] = {64, 8, C::kChunks, 2};
   const cuuint64_t vd[3] = {16, D, heads}, vs[2] = {32, D * 32};
   const cuuint32_t vb[3] = {16, D, 1};
+  const cuuint64_t qd[3] = {D, (cuuint64_t)a.Hq, (cuuint64_t)a.dims.T}, qs[2] = {D * 2, (cuuint64_t)a.Hq * D * 2};
+  a.tma_q = kTileRows % a.dims.Gq == 0;
+  const cuuint32_t qb[3] = {64, a.tma_q ? (cuuint32_t)a.dims.Gq : 1, a.tma_q ? (cuuint32_t)(kTileRows / a.dims.Gq) : 1};
+  const CUtensorMap tq = map_of(q, 3, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B);
   const CUtensorMap tk = map_of(k_cache, 4, kd, ks, kb, CU_TENSOR_MAP_SWIZZLE_128B);
   const CUtensorMap tv = map_of(v_cache, 3, vd, vs, vb, CU_TENSOR_MAP_SWIZZLE_32B);
   static bool attr[64] = {false};
@@ -1332,7 +1381,7 @@ static void launch_attn(const at::Tensor& k_cache, const at::Tensor& v_cache, At
     x.Hq = a.Hq, x.pages = a.pages, x.lean0 = lean0, x.scale_log2 = a.scale_log2, x.status = a.status;
     launch_k(attn_shared_lean_kernel<D>, a.dims.shares * 2, 128, 0, st, x);
   }
-  launch_k(attn_shared_kernel<D>, a.dims.shares, C::kThreads, C::kSmem, st, tk, tv, a);
+  launch_k(attn_shared_kernel<D>, a.dims.shares, C::kThreads, C::kSmem, st, tq, tk, tv, a);
   launch_k(attn_shared_merge_kernel<D>, (a.dims.T * a.Hq + 7) / 8, 256, 0, st, (const float*)a.part_o,
            (const float2*)a.part_ml, a.plan, a.dims, a.out, a.Hq, a.over, lean0);
 }
@@ -1382,9 +1431,9 @@ void attn_shared(const at::Tensor& q, const at::Tensor& k_cache, const at::Tenso
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.status = status_ptr(dev);
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  if (D == 64) launch_attn<64>(k_cache, v_cache, a, st, dev);
-  else if (D == 128) launch_attn<128>(k_cache, v_cache, a, st, dev);
-  else launch_attn<256>(k_cache, v_cache, a, st, dev);
+  if (D == 64) launch_attn<64>(q, k_cache, v_cache, a, st, dev);
+  else if (D == 128) launch_attn<128>(q, k_cache, v_cache, a, st, dev);
+  else launch_attn<256>(q, k_cache, v_cache, a, st, dev);
 }
 
 }  // namespace mb
