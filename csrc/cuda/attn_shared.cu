@@ -986,12 +986,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 }
 
 // ------------------------------------------------------------------------------------------------ lean
-// A sequence's own tokens for its few rows: HBM-bound, so what counts is many independent loads and little around them.
-// A warp owns a piece (16 rows, some pages) and needs no shared memory: the fragments of the 16 x 8 x 16 products are
-// loaded from the pages as they lie.  Both dimensions that are summed over are permuted for it: lane c of a quad takes
-// the head dims c D / 4 ... of Q and K in 16-byte loads (the same for both, so S is unchanged), and the tokens 4 c ...
-// 4 c + 3 of V's rows in 8-byte loads, which are the tokens whose S it holds.  The next page's K is loaded as soon as
-// S is computed, its V as soon as O is.  P enters the second product as two bf16 terms.
+// A sequence's own tokens for its few rows: HBM-bound, so what counts is bytes in flight and little around them.  A warp
+// owns a piece (16 rows, some pages) and a ring of pages of its own, each a bulk copy of K and one of V.  The fragments
+// of the 16 x 8 x 16 products are read as the pages lie: both dimensions that are summed over are permuted for it.  Lane
+// c of a quad takes the head dims 8 (4 i + c) ... + 7 of Q and K in 16-byte loads (the same for both, so S is
+// unchanged), and the tokens 4 c ... 4 c + 3 of V's rows in 8-byte loads, which are the tokens whose S it holds.  P
+// enters the second product as two bf16 terms.
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
   asm volatile(
@@ -1006,10 +1006,12 @@ __device__ __forceinline__ uint4 load16(const void* p) {
                : "l"(p));
   return r;
 }
-__device__ __forceinline__ uint2 load8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
+// An untiled copy of whole 16-byte units into this CTA's shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
@@ -1033,29 +1035,67 @@ struct LeanArgs {
   int* status;
 };
 
+constexpr int kLeanStages = 3;
+template <int D>
+constexpr int lean_smem() { return 4 * kLeanStages * D * 64 + 4 * kLeanStages * 8; }
+
 template <int D>
 __global__ void __launch_bounds__(128, 2) attn_shared_lean_kernel(const __grid_constant__ LeanArgs a) {
   constexpr int KS = D / 16, NT = D / 8, KV = D / 32;  // steps of S, column tiles of O, 16-byte loads of a K row's part
+  constexpr int ST = kLeanStages, kPage = D * 32;       // bytes of a page of K or V of a head
+  extern __shared__ __align__(128) uint8_t ring[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3, r = lane >> 2;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + 4 * ST * 2 * kPage) + warp * ST;
+  uint8_t* mine = ring + warp * ST * 2 * kPage;
+  const bool el = elect_one_sync();
+  if (lane == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, c = lane & 3, r = lane >> 2;
   const PlanView v = plan_view(a.plan, a.dims);
   const int Hkv = a.dims.Hkv, Gq = a.dims.Gq, items = v.hdr[3] * Hkv;
-  for (int item = (threadIdx.x >> 5) * gridDim.x + blockIdx.x; item < items; item += gridDim.x * 4) {
+  uint32_t asked = 0, taken = 0;  // pages, over all pieces
+  bool ok = true;
+  for (int item = warp * gridDim.x + blockIdx.x; item < items && ok; item += gridDim.x * 4) {
     const Piece x = reinterpret_cast<const Piece*>(v.lean)[item / Hkv];
     const int hk = item % Hkv;
     const int* bt = a.tables + (size_t)x.seq * a.dims.max_blocks + x.page0;
-    int ids = lane < x.pages ? bt[lane] : 0;
+    int ids = lane < x.pages ? bt[lane] : 0;  // of 32 pages
+    auto ask = [&](int i) {  // copies page i of the piece
+      if ((i & 31) == 0 && i) ids = i + lane < x.pages ? bt[i + lane] : 0;
+      const int id = __shfl_sync(~0u, ids, i & 31);
+      const uint32_t slot = asked % ST;
+      ++asked;
+      const size_t at = ((size_t)(id < 0 || id >= a.pages ? 0 : id) * Hkv + hk) * (16 * D);
+      if (el) {
+        mbar_arrive_expect_tx(&full[slot], 2 * kPage);
+        bulk_load(mine + slot * 2 * kPage, a.k + at, kPage, &full[slot]);
+        bulk_load(mine + slot * 2 * kPage + kPage, a.v + at, kPage, &full[slot]);
+      }
+      __syncwarp();
+    };
+    uint32_t bad = 0;  // pages of the piece, from the one that is taken next, that there is none of
+    auto check = [&](int i) {
+      if ((i & 31) == 0) {
+        const int id = i + lane < x.pages ? bt[i + lane] : 0;
+        bad = __ballot_sync(~0u, id < 0 || id >= a.pages);
+        if (bad) set_status(a.status, kErrBounds);
+      }
+      return (bad >> (i & 31)) & 1;
+    };
+    for (int i = 0; i < min(ST, x.pages); ++i) ask(i);
     const bool has0 = r < x.rows, has1 = r + 8 < x.rows;
     const int t0 = (x.row0 + r) / Gq, t1 = (x.row0 + r + 8) / Gq;
     const size_t o0 = ((size_t)t0 * a.Hq + hk * Gq + x.row0 + r - t0 * Gq) * D;
     const size_t o1 = ((size_t)t1 * a.Hq + hk * Gq + x.row0 + r + 8 - t1 * Gq) * D;
-    uint4 q0[KV], q1[KV], kr[2][KV];
-    uint2 vr[NT];
+    uint4 q0[KV], q1[KV];
 #pragma unroll
     for (int i = 0; i < KV; ++i) {
-      q0[i] = has0 ? load16(a.q + o0 + c * (D / 4) + i * 8) : make_uint4(0, 0, 0, 0);
-      q1[i] = has1 ? load16(a.q + o1 + c * (D / 4) + i * 8) : make_uint4(0, 0, 0, 0);
+      q0[i] = has0 ? load16(a.q + o0 + i * 32 + c * 8) : make_uint4(0, 0, 0, 0);
+      q1[i] = has1 ? load16(a.q + o1 + i * 32 + c * 8) : make_uint4(0, 0, 0, 0);
     }
     float acc[NT][4];
 #pragma unroll
@@ -1064,49 +1104,27 @@ __global__ void __launch_bounds__(128, 2) attn_shared_lean_kernel(const __grid_c
     // keys of this lane in a page: 4 c + {0, 1, 2, 3}; row r sees those below lim
     const int base = x.page0 * 16 + 4 * c;
     const int lim0 = min(x.ctx, x.lim + t0), lim1 = min(x.ctx, x.lim + t1);
-    const int tk = 4 * (r >> 1) + (r & 1);  // the token of K that this lane loads for the first column tile; + 2: the second
-    int page = 0;
-    auto next_page = [&](int i) {  // -1: no such page
-      if ((i & 31) == 0 && i) ids = i + lane < x.pages ? bt[i + lane] : 0;
-      int p = __shfl_sync(~0u, ids, i & 31);
-      if (p < 0 || p >= a.pages) {
-        set_status(a.status, kErrBounds);
-        p = -1;
-      }
-      return p;
-    };
-    auto load_k = [&](int p) {
-      const __nv_bfloat16* k = a.k + (((size_t)max(p, 0) * Hkv + hk) * 16 + tk) * D + c * (D / 4);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < KV; ++i) kr[j][i] = load16(k + j * 2 * D + i * 8);
-    };
-    auto load_v = [&](int p) {
-      const __nv_bfloat16* w = a.v + (((size_t)max(p, 0) * Hkv + hk) * D + r) * 16 + 4 * c;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) vr[i] = load8(w + i * 128);
-    };
-    page = next_page(0);
-    load_k(page);
-    load_v(page);
-    for (int i = 0; i < x.pages; ++i) {
+    const int tk = 4 * (r >> 1) + (r & 1);  // the token of K that this lane reads for the first column tile; + 2: the second
+    for (int i = 0; i < x.pages; ++i, ++taken) {
+      const bool gone = check(i);
+      const uint32_t slot = taken % ST;
+      ok = __all_sync(~0u, bar_wait(&full[slot], (taken / ST) & 1, a.status));
+      if (!ok) break;
+      const uint8_t* kp = mine + slot * 2 * kPage + tk * D * 2 + c * 16;
+      const uint8_t* vp = mine + slot * 2 * kPage + kPage + r * 32 + c * 8;
       float s[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-        for (int t = 0; t < KS / 2; ++t) {
-          mma_16816(s[j], q0[t].x, q1[t].x, q0[t].y, q1[t].y, kr[j][t].x, kr[j][t].y);
-          mma_16816(s[j], q0[t].z, q1[t].z, q0[t].w, q1[t].w, kr[j][t].z, kr[j][t].w);
+        for (int t = 0; t < KV; ++t) {
+          const uint4 k = *reinterpret_cast<const uint4*>(kp + j * 4 * D + t * 64);
+          mma_16816(s[j], q0[t].x, q1[t].x, q0[t].y, q1[t].y, k.x, k.y);
+          mma_16816(s[j], q0[t].z, q1[t].z, q0[t].w, q1[t].w, k.z, k.w);
         }
       }
-      const int now = page, key = base + i * 16;
-      if (i + 1 < x.pages) {
-        page = next_page(i + 1);
-        load_k(page);
-      }
-      const int seen0 = now < 0 ? 0 : lim0 - key, seen1 = now < 0 ? 0 : lim1 - key;
+      const int key = base + i * 16;
+      const int seen0 = gone ? 0 : lim0 - key, seen1 = gone ? 0 : lim1 - key;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -1144,19 +1162,21 @@ __global__ void __launch_bounds__(128, 2) attn_shared_lean_kernel(const __grid_c
                                     y[2 * e + 1] - __uint_as_float(hi[2 * j + e] & 0xffff0000u));
         }
       }
-      if (now < 0 || key - 4 * c + 16 > x.ctx) {  // token slots past the context may hold anything
-        const int left = now < 0 ? 0 : x.ctx - key;
-        const uint32_t k0 = left >= 2 ? ~0u : left == 1 ? 0xffffu : 0u, k1 = left >= 4 ? ~0u : left == 3 ? 0xffffu : 0u;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) vr[t].x &= k0, vr[t].y &= k1;
-      }
+      // token slots past the context may hold anything
+      const int left = gone ? 0 : x.ctx - key;
+      const uint32_t k0 = left >= 2 ? ~0u : left == 1 ? 0xffffu : 0u, k1 = left >= 4 ? ~0u : left == 3 ? 0xffffu : 0u;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        mma_16816(acc[t], hi[0], hi[1], hi[2], hi[3], vr[t].x, vr[t].y);
-        mma_16816(acc[t], lo[0], lo[1], lo[2], lo[3], vr[t].x, vr[t].y);
+        uint2 y = *reinterpret_cast<const uint2*>(vp + t * 256);
+        y.x &= k0;
+        y.y &= k1;
+        mma_16816(acc[t], hi[0], hi[1], hi[2], hi[3], y.x, y.y);
+        mma_16816(acc[t], lo[0], lo[1], lo[2], lo[3], y.x, y.y);
       }
-      if (i + 1 < x.pages) load_v(page);
+      __syncwarp();  // the page has been read
+      if (i + ST < x.pages) ask(i + ST);
     }
+    if (!ok) break;
     l0 = quad_sum(l0);
     l1 = quad_sum(l1);
     if (x.direct) {
@@ -1178,6 +1198,8 @@ __global__ void __launch_bounds__(128, 2) attn_shared_lean_kernel(const __grid_c
       }
     }
   }
+  // no copy may be in flight when the CTA leaves
+  for (; taken < asked; ++taken) bar_wait(&full[taken % ST], (taken / ST) & 1, a.status);
 }
 
 // Joins the partials of a row (a warp each) and writes the rows that no unit covers as zeros.
@@ -1379,7 +1401,13 @@ static void launch_attn(const at::Tensor& q, const at::Tensor& k_cache, const at
     x.v = reinterpret_cast<const __nv_bfloat16*>(v_cache.data_ptr());
     x.tables = a.tables, x.out = a.out, x.part_o = a.part_o, x.part_ml = a.part_ml, x.plan = a.plan, x.dims = a.dims;
     x.Hq = a.Hq, x.pages = a.pages, x.lean0 = lean0, x.scale_log2 = a.scale_log2, x.status = a.status;
-    launch_k(attn_shared_lean_kernel<D>, a.dims.shares * 2, 128, 0, st, x);
+    static bool attr[64] = {false};
+    if (!attr[dev]) {
+      C10_CUDA_CHECK(cudaFuncSetAttribute(attn_shared_lean_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          lean_smem<D>()));
+      attr[dev] = true;
+    }
+    launch_k(attn_shared_lean_kernel<D>, a.dims.shares * 2, 128, lean_smem<D>(), st, x);
   }
   launch_k(attn_shared_kernel<D>, a.dims.shares, C::kThreads, C::kSmem, st, tq, tk, tv, a);
   launch_k(attn_shared_merge_kernel<D>, (a.dims.T * a.Hq + 7) / 8, 256, 0, st, (const float*)a.part_o,
