@@ -150,7 +150,8 @@ void kv_compact(const std::vector<at::Tensor>& k, const std::vector<at::Tensor>&
 void verify_sampled(const at::Tensor& logits, const at::Tensor& cu, const at::Tensor& drafts,
                     const at::Tensor& uniforms, const at::Tensor& noise, const at::Tensor& temperature,
                     const c10::optional<at::Tensor>& draft_probs, at::Tensor& accepted, at::Tensor& token,
-                    at::Tensor& probs);
+                    at::Tensor& probs, at::Tensor& workspace);
+int64_t verify_sampled_ws(int64_t B, int64_t K, int64_t V);
 }  // namespace mb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -221,5 +222,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_copy_pages", &mb::kv_copy_pages);
   m.def("kv_compact", &mb::kv_compact);
   m.def("verify_sampled", &mb::verify_sampled);
+  m.def("verify_sampled_ws", &mb::verify_sampled_ws);
   m.def("read_and_clear_status", &mb::read_and_clear_status);
 }

@@ -297,7 +297,8 @@ def verify_sampled(logits, cu, drafts, uniforms, noise, temperature, draft_probs
     accepted = torch.empty(B, dtype=torch.int32, device=dev)
     token = torch.empty(B, dtype=torch.int64, device=dev)
     probs = torch.empty(B, K + 1, dtype=torch.float32, device=dev)
-    _C().verify_sampled(logits, cu, drafts, uniforms, noise, temperature, draft_probs, accepted, token, probs)
+    ws = torch.empty(_C().verify_sampled_ws(B, K, logits.shape[1]), dtype=torch.uint8, device=dev)
+    _C().verify_sampled(logits, cu, drafts, uniforms, noise, temperature, draft_probs, accepted, token, probs, ws)
     return accepted, token, probs
 
 
