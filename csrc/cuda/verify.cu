@@ -8,15 +8,17 @@
 // temperature <= 0: p_j is 1 at the row's largest logit (lowest id among equals).
 // NaN logits count as -inf; rows without a finite or +inf logit accept nothing and give token -1.
 //
-// Bound by HBM: every logit is read once for its row's largest value and sum of exponentials (a CTA for each part of a
-// row, its values in registers between the two), and of each sequence one row more with its noise (and q) for the next
-// token.  Two launches:
-//   rows:  (largest logit, its lowest id, sum of exp((x - largest) / temperature)) of each part of each row;
+// Bound by HBM: every logit is read once for its row's largest value and sum of exponentials, and of each sequence one
+// row more with its noise (and q) for the next token.  Two launches, each of which cuts its rows into as many parts as
+// fill the GPU, a CTA each:
+//   rows:  (largest logit, its lowest id, sum of exp((x - largest) / temperature)) of each part of each row, with a running
+//          maximum and sum in every thread and one reduction in the end;
 //   token: every CTA joins its sequence's parts and decides on the drafts, as all CTAs of the sequence do alike, then
 //          takes its part of the row that the next token is drawn from; the last one of the sequence joins the parts.
-// A draw compares r / noise of all ids.  Approximate bounds of it (2^-16 either way) leave a handful of candidates in a
-// part, and only those are computed with the correctly rounded divisions and the full exponential that the outcome is
-// defined by: three divisions for each id would take longer than reading it.  Sums are in fp32.
+// A draw compares r / noise of all ids.  Each thread keeps approximate bounds of it (2^-16 either way): its largest
+// upper bound with the id, the second largest, and the largest lower bound.  An id below its part's largest lower bound
+// is out, so that one or two are left, and only those are computed with the correctly rounded divisions and the full
+// exponential that the outcome is defined by: three divisions for each id take longer than reading it.  Sums are in fp32.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -34,70 +36,65 @@ constexpr int kMaxDrafts = 1023;
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// Part `part` of row[0..V): the values at ids id(k, e) in registers, `outside` where there is no id.  Aligned 16-byte
-// loads wherever a whole vector lies in the row; the row may begin anywhere.
-template <typename T, int VECS>
-struct Part {
-  static constexpr int kVec = 16 / sizeof(T), kIds = kThreads * VECS * kVec;
-  float x[VECS * kVec];
-  int first;  // id of x[0]; the next vector is kThreads * kVec ids on
-  __device__ __forceinline__ int id(int i) const { return first + (i / kVec) * (kThreads * kVec) + i % kVec; }
-  __device__ __forceinline__ void load(const T* row, int V, int part, float outside) {
-    const int skew = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % kVec);
-    first = part * kIds + threadIdx.x * kVec - skew;
-    uint4 raw[VECS];
-#pragma unroll
-    for (int k = 0; k < VECS; ++k) {
-      const int v = id(k * kVec);
-      if (v >= 0 && v + kVec <= V) raw[k] = __ldg(reinterpret_cast<const uint4*>(row + v));
-    }
-#pragma unroll
-    for (int k = 0; k < VECS; ++k) {
-      const int v = id(k * kVec);
-      const T* y = reinterpret_cast<const T*>(&raw[k]);
-      if (v >= 0 && v + kVec <= V) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) x[k * kVec + e] = to_f(y[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) x[k * kVec + e] = v + e >= 0 && v + e < V ? to_f(row[v + e]) : outside;
+// N neighbouring values, loaded as 16-byte vectors (8 bytes of four bf16).  Loading and looking are apart so that the
+// loads of several are under way together.
+template <int N, typename X>
+struct Vec {
+  static constexpr int kWords = N * (int)sizeof(X) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const X* p, bool ok) {
+    if constexpr (kWords == 2) {
+      if (ok) {
+        const uint2 y = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = y.x, w[1] = y.y;
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4)
+        if (ok) {
+          const uint4 y = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+          w[i] = y.x, w[i + 1] = y.y, w[i + 2] = y.z, w[i + 3] = y.w;
+        }
     }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(X) == 4) return __uint_as_float(w[e]);
+    else return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+  }
+  static __device__ __forceinline__ bool aligned(const X* p) {
+    return reinterpret_cast<uintptr_t>(p) % (kWords == 2 ? 8 : 16) == 0;
+  }
+};
+// p[v .. v + N) one by one, `outside` where [0, end) does not reach.
+template <int N, typename X>
+__device__ __forceinline__ void load_each(const X* p, int v, int end, float outside, float (&x)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = v + e >= 0 && v + e < end ? to_f(p[v + e]) : outside;
+}
+
+// A thread's ids of part `part` of a row: kIds = 16 bytes' worth from each of at(0), at(1), ... while they are below end.
+// The vectors lie on 16-byte boundaries wherever the row begins.
+template <typename T>
+struct Span {
+  static constexpr int kIds = 16 / sizeof(T), kStep = kThreads * kIds;
+  int first, end;
+  __device__ __forceinline__ Span(const T* row, int V, int part, int steps) {
+    const int skew = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % kIds);
+    first = part * steps * kStep + threadIdx.x * kIds - skew;
+    end = min(V, (part + 1) * steps * kStep - skew);
   }
 };
 
-// p[v0 .. v0 + N) within p[0..V): in 16-byte loads (8 bytes of four bf16) where they are aligned.
-template <int N, typename X>
-__device__ __forceinline__ void load_some(const X* p, int v0, int V, float (&out)[N]) {
-  constexpr int kBytes = N * sizeof(X) < 16 ? 8 : 16, kPer = kBytes / sizeof(X);
-  if (v0 >= 0 && v0 + N <= V && reinterpret_cast<uintptr_t>(p + v0) % kBytes == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += kPer) {
-      uint4 raw;
-      if constexpr (kBytes == 16) {
-        raw = __ldg(reinterpret_cast<const uint4*>(p + v0 + i));
-      } else {
-        const uint2 half = __ldg(reinterpret_cast<const uint2*>(p + v0 + i));
-        raw = make_uint4(half.x, half.y, 0, 0);
-      }
-      const X* y = reinterpret_cast<const X*>(&raw);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) out[i + e] = to_f(y[e]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) out[e] = v0 + e >= 0 && v0 + e < V ? to_f(p[v0 + e]) : 1.f;
-  }
+// Steps (of a CTA's 4 KB) a part and parts a row for `rows` rows of V ids: parts that fill `ctas` places once.
+template <typename T>
+void cut(int64_t V, int64_t rows, int64_t ctas, int& steps, int& parts) {
+  const int64_t all = (V + Span<T>::kIds - 1 + Span<T>::kStep - 1) / Span<T>::kStep;  // a row may begin inside a vector
+  const int64_t want = std::min(all, std::max<int64_t>(1, ctas / std::max<int64_t>(1, rows)));
+  steps = (int)((all + want - 1) / want);
+  parts = (int)((all + steps - 1) / steps);
 }
 
-// Parts of a row of V ids, wherever it begins.
-template <typename T, int VECS>
-int parts_of(int64_t V) {
-  using P = Part<T, VECS>;
-  return (int)((V + P::kVec - 1 + P::kIds - 1) / P::kIds);
-}
-
-__device__ __forceinline__ float no_nan(float x) { return x != x ? -INFINITY : x; }
+__device__ __forceinline__ float no_nan(float x) { return fmaxf(x, -INFINITY); }
 
 // exp((x - top) / temperature); a row whose top is +inf spreads its mass over the infinite logits
 __device__ __forceinline__ float weight(float x, float top, float heat) {
@@ -106,6 +103,12 @@ __device__ __forceinline__ float weight(float x, float top, float heat) {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float ex2_ftz(float x) {  // without results below 2^-126, one instruction
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -138,8 +141,8 @@ struct RowPart {
   int pad;
 };
 struct TokenPart {
-  float s[2];  // best of the rest of p, best of p
-  int v[2];
+  float s;  // the best score and its id
+  int v;
 };
 
 struct VerifyArgs {
@@ -154,7 +157,7 @@ struct VerifyArgs {
   RowPart* rows;      // [B, K + 1, parts]
   TokenPart* tokens;  // [B, parts]
   int* done;          // [B]
-  int B, K, V, num_rows, row_parts, token_parts;
+  int B, K, V, num_rows, row_steps, row_parts, token_steps, token_parts;
   int* status;
 };
 
@@ -164,41 +167,81 @@ __device__ __forceinline__ int2 rows_of(const VerifyArgs& a, int b) {
   return make_int2(r0, r0 < 0 || n < 0 || n > a.K || r0 + n >= a.num_rows ? -1 : n);
 }
 
-template <typename T, int VECS>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const __grid_constant__ VerifyArgs a) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const __grid_constant__ VerifyArgs a) {
   __shared__ float sh[kWarps];
   __shared__ int at;
   pdl_wait();
   pdl_trigger();
   const int part = blockIdx.x, j = blockIdx.y, b = blockIdx.z;
   if (part == 0 && j == 0 && threadIdx.x == 0) a.done[b] = 0;
+  const float heat = a.temperature[b];
   const int2 r = rows_of(a, b);
   if (j > r.y) return;
-  Part<T, VECS> p;
-  p.load(static_cast<const T*>(a.logits) + (size_t)(r.x + j) * a.V, a.V, part, -INFINITY);
-  const float heat = a.temperature[b];
   if (threadIdx.x == 0) at = INT_MAX;
-  float top = -INFINITY;
+  const T* row = static_cast<const T*>(a.logits) + (size_t)(r.x + j) * a.V;
+  const Span<T> ids(row, a.V, part, a.row_steps);
+  constexpr int N = Span<T>::kIds, kStep = Span<T>::kStep, kDeep = 4;
+  const bool greedy = !(heat > 0.f);
+  const float f = greedy ? 0.f : 1.4426950408889634f / heat;
+  float top = -INFINITY, sum = 0.f;
+  int mine = INT_MAX;
+  for (int v0 = ids.first; v0 < ids.end; v0 += kDeep * kStep) {
+    Vec<N, T> raw[kDeep];
+    bool in[kDeep];
 #pragma unroll
-  for (int i = 0; i < VECS * p.kVec; ++i) {
-    p.x[i] = no_nan(p.x[i]);
-    top = fmaxf(top, p.x[i]);
-  }
-  const float mine = top;
-  top = block_max(top, sh);
-  float sum = 0.f;
-  if (heat > 0.f) {
-    if (top != -INFINITY) {
-      const float f = 1.4426950408889634f / heat;
-#pragma unroll
-      for (int i = 0; i < VECS * p.kVec; ++i) sum += p.x[i] == top ? 1.f : ex2((p.x[i] - top) * f);
+    for (int k = 0; k < kDeep; ++k) {
+      const int v = v0 + k * kStep;
+      in[k] = v >= 0 && v + N <= ids.end;
+      raw[k].load(row + v, in[k]);
     }
-  } else if (mine == top && top != -INFINITY) {  // greedy: the lowest id is wanted, no sum
-    int v = INT_MAX;
+    float x[kDeep][N];
 #pragma unroll
-    for (int i = 0; i < VECS * p.kVec; ++i)
-      if (p.x[i] == top) v = min(v, p.id(i));
-    atomicMin(&at, v);
+    for (int k = 0; k < kDeep; ++k) {
+      const int v = v0 + k * kStep;
+      if (!in[k]) {  // the row's ends
+        load_each<N>(row, v, v < ids.end ? ids.end : 0, -INFINITY, x[k]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[k][e] = no_nan(x[k][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[k][e] = no_nan(raw[k].get(e));
+      }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e) m = fmaxf(m, x[k][e]);
+    if (m == -INFINITY) continue;
+    if (greedy) {
+      if (m > top) {
+        top = m;
+#pragma unroll
+        for (int k = kDeep - 1; k >= 0; --k)
+#pragma unroll
+          for (int e = N - 1; e >= 0; --e)
+            if (x[k][e] == m) mine = v0 + k * kStep + e;
+      }
+      continue;
+    }
+    if (m > top) {
+      sum *= ex2((top - m) * f);
+      top = m;
+    }
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        s[e & 3] += top == INFINITY ? (x[k][e] == top ? 1.f : 0.f) : ex2_ftz((x[k][e] - top) * f);
+    sum += (s[0] + s[1]) + (s[2] + s[3]);
+  }
+  const float all = block_max(top, sh);
+  if (greedy) {
+    if (top == all && mine != INT_MAX) atomicMin(&at, mine);
+  } else {
+    sum = top == all || top == -INFINITY ? sum : sum * ex2((top - all) * f);
   }
   sum = warp_sum(sum);
   __syncthreads();
@@ -207,12 +250,12 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const __grid_cons
   if (threadIdx.x == 0) {
     sum = 0.f;
     for (int w = 0; w < kWarps; ++w) sum += sh[w];
-    a.rows[((size_t)b * (a.K + 1) + j) * a.row_parts + part] = {top, at, sum, 0};
+    a.rows[((size_t)b * (a.K + 1) + j) * a.row_parts + part] = {all, at, sum, 0};
   }
 }
 
-template <typename T, typename Q, int VECS>
-__global__ void __launch_bounds__(kThreads) verify_token_kernel(const __grid_constant__ VerifyArgs a) {
+template <typename T, typename Q>
+__global__ void __launch_bounds__(kThreads, 3) verify_token_kernel(const __grid_constant__ VerifyArgs a) {
   extern __shared__ float dyn[];  // [K + 1] of each: largest logit, sum, p of the draft; lowest id of the largest
   float *tops = dyn, *sums = tops + a.K + 1, *pds = sums + a.K + 1;
   int* ats = reinterpret_cast<int*>(pds + a.K + 1);
@@ -285,90 +328,149 @@ __global__ void __launch_bounds__(kThreads) verify_token_kernel(const __grid_con
   const int64_t d = refused ? a.drafts[(size_t)b * a.K + k] : -1;
   const Q* q = refused && probs ? probs + ((size_t)b * a.K + k) * a.V : nullptr;
   // the next token: from the rest of p where a draft was refused, else (or where nothing is left) from p
-  float s1 = 0.f, s2 = 0.f;
-  int v1 = INT_MAX, v2 = INT_MAX;
-  auto precise = [&](float x, int v) {
-    const float p = p_of(x, v, k), z = noise[v];
-    if (p > 0.f) better(s2, v2, __fdiv_rn(p, z), v);
-    if (refused) {
-      const float rest = p - (q ? to_f(q[v]) : v == d ? 1.f : 0.f);
-      if (rest > 0.f) better(s1, v1, __fdiv_rn(rest, z), v);
-    }
+  float best = 0.f;
+  int at = INT_MAX;
+  auto precise = [&](int v, bool rest) {
+    float p = p_of(to_f(row[v]), v, k);
+    if (rest) p -= q ? to_f(q[v]) : v == d ? 1.f : 0.f;
+    if (p > 0.f) better(best, at, __fdiv_rn(p, noise[v]), v);
   };
   if (greedy) {
-    if (!empty && part == 0 && tid == 0) precise(top, ats[k]);  // p is elsewhere 0
+    if (!empty && part == 0 && tid == 0) precise(ats[k], refused);  // p is elsewhere 0
   } else if (!empty) {
-    Part<T, VECS> x;
-    constexpr int NV = Part<T, VECS>::kVec, N = VECS * NV;
-    static_assert(N <= 32, "a candidate is a bit");
-    x.load(row, a.V, part, -INFINITY);
-    constexpr float kUp = 1.f + 1.f / 65536, kDown = 1.f - 1.f / 65536;
-    const float f = 1.4426950408889634f / heat, g = 1.f / sum;
-    float hi1[N], hi2[N], lo1 = 0.f, lo2 = 0.f;  // bounds of the scores of the rest and of p
+    const Span<T> ids(row, a.V, part, a.token_steps);
+    constexpr int N = Span<T>::kIds, kStep = Span<T>::kStep;
+    constexpr float kUp = 1.f + 1.f / 65536, kDown = 1.f - 1.f / 65536, kTiny = 1.2e-38f;
+    const float f = 1.4426950408889634f / heat;
+    const bool z_ok = Vec<N, float>::aligned(noise + ids.first), q_ok = q && Vec<N, Q>::aligned(q + ids.first);
+    float up1 = 0.f, up2 = 0.f, low = 0.f;  // the two largest upper bounds, the largest lower one
+    int id1 = -1;
+    // `take` sees N ids from v on with their logits and noise; where the row does not reach, -inf and 1
+    auto each = [&](auto take) {
+      constexpr int kDeep = 2;
+      for (int v0 = ids.first; v0 < ids.end; v0 += kDeep * kStep) {
+        Vec<N, T> raw[kDeep];
+        Vec<N, float> zs[kDeep];
+        bool in[kDeep];
 #pragma unroll
-    for (int i = 0; i < N; i += NV) {
-      const int v0 = x.id(i);
-      float z[NV], qv[NV];
-      load_some<NV>(noise, v0, a.V, z);
-      if (q) load_some<NV>(q, v0, a.V, qv);
+        for (int k = 0; k < kDeep; ++k) {
+          const int v = v0 + k * kStep;
+          in[k] = v >= 0 && v + N <= ids.end;
+          raw[k].load(row + v, in[k]);
+          zs[k].load(noise + v, in[k] && z_ok);
+        }
 #pragma unroll
-      for (int e = 0; e < NV; ++e) {
-        const int v = v0 + e;
-        const float y = no_nan(x.x[i + e]);
-        hi1[i + e] = hi2[i + e] = -1.f;
-        if (v >= 0 && v < a.V) {
-          const float p = (y == top ? 1.f : ex2((y - top) * f)) * g, w = __fdividef(1.f, z[e]);
-          hi2[i + e] = p * w * (kUp * kUp);
-          lo2 = fmaxf(lo2, p * w * (kDown * kDown));
-          if (refused) {
-            const float t = q ? qv[e] : v == d ? 1.f : 0.f;
-            hi1[i + e] = fmaxf(p * kUp - t, 0.f) * w * kUp;
-            lo1 = fmaxf(lo1, (p * kDown - t) * w * kDown);
+        for (int k = 0; k < kDeep; ++k) {
+          const int v = v0 + k * kStep, end = v < ids.end ? ids.end : 0;
+          float x[N], z[N];
+          if (in[k]) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = raw[k].get(e);
+          } else {
+            load_each<N>(row, v, end, -INFINITY, x);
           }
+          if (in[k] && z_ok) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) z[e] = zs[k].get(e);
+          } else {
+            load_each<N>(noise, v, end, 1.f, z);
+          }
+          take(v, end, in[k], x, z);
         }
       }
-    }
-    lo2 = block_max(lo2, sh);
-    lo1 = refused ? block_max(lo1, sh) : 0.f;
-    // bounds this small say nothing (a rest that is all rounding, weights next to underflow): everything is a candidate
-    if (!(lo1 > 1e-30f)) lo1 = 0.f;
-    if (!(lo2 > 1e-30f)) lo2 = 0.f;
-    uint32_t candidates = 0;  // of p too where a draft was refused: whether its rest is empty is known in the end
+    };
+    if (!q) {
+      // p but for its factor: 2^(60 + ...) keeps every p that is not zero in 32 bits above the flush to zero
+      const int only = refused && d >= 0 && d < a.V ? (int)d : -1;  // a certain draft's rest: p elsewhere
+      each([&](int v, int, bool, float (&x)[N], float (&z)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) candidates |= (uint32_t)(hi2[i] >= lo2 || (refused && hi1[i] >= lo1)) << i;
-#pragma unroll 1
-    for (; candidates; candidates &= candidates - 1) {
-      const int v = x.id(__ffs(candidates) - 1);
-      precise(to_f(row[v]), v);
+        for (int e = 0; e < N; ++e) {
+          float p = ex2_ftz(fmaf(no_nan(x[e]) - top, f, 60.f));
+          if (top == INFINITY) p = x[e] == top ? 1.f : 0.f;
+          const float s = v + e == only ? 0.f : p * __fdividef(1.f, z[e]);
+          up2 = fmaxf(up2, fminf(s, up1));
+          if (s > up1) id1 = v + e;
+          up1 = fmaxf(up1, s);
+        }
+      });
+      const float g = (top == INFINITY ? 1.f : 0x1p-60f) / sum;
+      low = up1 * g * (kDown * kDown);
+      up1 *= g * (kUp * kUp);
+      up2 *= g * (kUp * kUp);
+    } else {
+      const float g = 1.f / sum;
+      each([&](int v, int end, bool in, float (&x)[N], float (&z)[N]) {
+        float t[N];
+        if (in && q_ok) {
+          Vec<N, Q> qs;
+          qs.load(q + v, true);
+#pragma unroll
+          for (int e = 0; e < N; ++e) t[e] = qs.get(e);
+        } else {
+          load_each<N>(q, v, end, 2.f, t);  // 2: outside, nothing is left
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float y = no_nan(x[e]), w = __fdividef(1.f, z[e]);
+          const float p = (y == top ? 1.f : ex2_ftz((y - top) * f)) * g;
+          const float s = fmaxf(fmaf(p, kUp, kTiny) - t[e], 0.f) * w * kUp;  // kTiny: a p that was flushed to zero
+          low = fmaxf(low, (p * kDown - t[e]) * w * kDown);
+          up2 = fmaxf(up2, fminf(s, up1));
+          if (s > up1) id1 = v + e;
+          up1 = fmaxf(up1, s);
+        }
+      });
+    }
+    const float most = block_max(up1, sh);
+    low = block_max(low, sh);
+    // Bounds near underflow say nothing.  Such a part has no winner where the row's largest logit is in the race, whose
+    // score is at least 1 / (V noise); else (it was refused, or q leaves rounding only) every id of it is computed.
+    const bool top_runs = !refused || (!q && !(d >= 0 && d < a.V && to_f(row[d]) == top));
+    if (most == 0.f || (!(low > 1e-30f) && top_runs)) {
+    } else if (!(low > 1e-30f) || up2 >= low) {
+      for (int v0 = ids.first; v0 < ids.end; v0 += kStep)
+        for (int v = max(v0, 0); v < min(v0 + N, ids.end); ++v) precise(v, refused);
+    } else if (up1 >= low) {
+      precise(id1, refused);
     }
   }
-  warp_better(s1, v1);
-  warp_better(s2, v2);
-  if (lane == 0) best_of[warp] = {{s1, s2}, {v1, v2}};
+  warp_better(best, at);
+  if (lane == 0) best_of[warp] = {best, at};
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) {
-      better(s1, v1, best_of[w].s[0], best_of[w].v[0]);
-      better(s2, v2, best_of[w].s[1], best_of[w].v[1]);
-    }
-    a.tokens[(size_t)b * a.token_parts + part] = {{s1, s2}, {v1, v2}};
+    for (int w = 1; w < kWarps; ++w) better(best, at, best_of[w].s, best_of[w].v);
+    a.tokens[(size_t)b * a.token_parts + part] = {best, at};
     __threadfence();
     last = atomicAdd(&a.done[b], 1) == a.token_parts - 1;
   }
   __syncthreads();
   if (!last) return;
   __threadfence();
-  if (warp == 0) {
-    s1 = s2 = 0.f;
-    v1 = v2 = INT_MAX;
+  best = 0.f;
+  at = INT_MAX;
+  if (tid < 32) {
     for (int i = lane; i < a.token_parts; i += 32) {
       const TokenPart x = a.tokens[(size_t)b * a.token_parts + i];
-      better(s1, v1, x.s[0], x.v[0]);
-      better(s2, v2, x.s[1], x.v[1]);
+      better(best, at, x.s, x.v);
     }
-    warp_better(s1, v1);
-    warp_better(s2, v2);
-    const int v = v1 < INT_MAX ? v1 : v2 < INT_MAX ? v2 : -1;
+    warp_better(best, at);
+    if (lane == 0) best_of[0] = {best, at};
+  }
+  __syncthreads();
+  if (best_of[0].v == INT_MAX && refused && !empty) {  // q took all of p: the whole row again, from p
+    best = 0.f;
+    at = INT_MAX;
+    for (int v = tid; v < a.V; v += kThreads) precise(v, false);
+    warp_better(best, at);
+    __syncthreads();
+    if (lane == 0) best_of[warp] = {best, at};
+    __syncthreads();
+    if (tid == 0)
+      for (int w = 1; w < kWarps; ++w) better(best_of[0].s, best_of[0].v, best_of[w].s, best_of[w].v);
+    __syncthreads();
+  }
+  if (warp == 0) {
+    const int v = best_of[0].v < INT_MAX ? best_of[0].v : -1;
     if (lane == 0) {
       a.accepted[b] = k;
       a.token[b] = v;
@@ -381,9 +483,9 @@ __global__ void __launch_bounds__(kThreads) verify_token_kernel(const __grid_con
 
 }  // namespace
 
-// Bytes of workspace: parts of the smallest size, whatever the types.
+// Bytes of workspace, whatever the types: parts of 4 KB.
 int64_t verify_sampled_ws(int64_t B, int64_t K, int64_t V) {
-  const int64_t parts = std::max(parts_of<float, 2>(V), parts_of<__nv_bfloat16, 1>(V));
+  const int64_t parts = (V + 1024 + 8) / 1024 + 1;
   return B * ((K + 1) * parts * (int64_t)sizeof(RowPart) + parts * (int64_t)sizeof(TokenPart) + 16);
 }
 
@@ -436,43 +538,25 @@ void verify_sampled(const at::Tensor& logits, const at::Tensor& cu, const at::Te
   a.accepted = accepted.data_ptr<int>(), a.token = token.data_ptr<int64_t>(), a.probs = probs.data_ptr<float>();
   a.B = (int)B, a.K = (int)K, a.V = (int)V, a.num_rows = (int)logits.size(0);
   a.status = status_ptr(logits.device().index());
-  // large parts where they fill the GPU twice, small ones where there are few rows
-  auto rows = [&](auto* t, auto vecs) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    constexpr int VECS = decltype(vecs)::value;
-    a.row_parts = parts_of<T, VECS>(V);
-    launch_k(verify_rows_kernel<T, VECS>, dim3(a.row_parts, (unsigned)(K + 1), (unsigned)B), kThreads, 0, st, a);
-  };
-  auto tokens = [&](auto* t, auto* qt, auto vecs) {
+  auto go = [&](auto* t, auto* qt) {
     using T = std::remove_pointer_t<decltype(t)>;
     using Q = std::remove_pointer_t<decltype(qt)>;
-    constexpr int VECS = decltype(vecs)::value;
-    a.token_parts = parts_of<T, VECS>(V);
-    launch_k(verify_token_kernel<T, Q, VECS>, dim3(a.token_parts, (unsigned)B), kThreads, (size_t)(16 * (K + 1)), st, a);
-  };
-  auto go = [&](auto* t, auto* qt, auto small, auto large) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    // one region for both sizes of parts
-    const int64_t most = parts_of<T, decltype(small)::value>(V);
+    // as many CTAs as are resident: four an SM for the rows, three for the token, whose threads hold more
+    cut<T>(V, a.num_rows, 4 * sms, a.row_steps, a.row_parts);
+    cut<T>(V, B, 3 * sms, a.token_steps, a.token_parts);
     uint8_t* ws = static_cast<uint8_t*>(workspace.data_ptr());
     a.rows = reinterpret_cast<RowPart*>(ws);
-    a.tokens = reinterpret_cast<TokenPart*>(ws + B * (K + 1) * most * (int64_t)sizeof(RowPart));
-    a.done = reinterpret_cast<int*>(a.tokens + B * most);
-    const int64_t wide = parts_of<T, decltype(large)::value>(V);
-    if ((int64_t)a.num_rows * wide >= 2 * sms) rows(t, large);
-    else rows(t, small);
-    if (B * wide >= 2 * sms) tokens(t, qt, large);
-    else tokens(t, qt, small);
+    a.tokens = reinterpret_cast<TokenPart*>(a.rows + B * (K + 1) * a.row_parts);
+    a.done = reinterpret_cast<int*>(a.tokens + B * a.token_parts);
+    launch_k(verify_rows_kernel<T>, dim3(a.row_parts, (unsigned)(K + 1), (unsigned)B), kThreads, 0, st, a);
+    launch_k(verify_token_kernel<T, Q>, dim3(a.token_parts, (unsigned)B), kThreads, (size_t)(16 * (K + 1)), st, a);
   };
-  auto with_q = [&](auto* t, auto small, auto large) {
-    if (draft_probs && draft_probs->scalar_type() == at::kBFloat16) go(t, (__nv_bfloat16*)nullptr, small, large);
-    else go(t, (float*)nullptr, small, large);
+  auto with_q = [&](auto* t) {
+    if (draft_probs && draft_probs->scalar_type() == at::kBFloat16) go(t, (__nv_bfloat16*)nullptr);
+    else go(t, (float*)nullptr);
   };
-  // vectors a thread: 8 or 32 ids of bf16 (2 or 8 KB a part), 8 or 16 of fp32 (8 or 16 KB)
-  if (logits.scalar_type() == at::kBFloat16)
-    with_q((__nv_bfloat16*)nullptr, std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
-  else
-    with_q((float*)nullptr, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+  if (logits.scalar_type() == at::kBFloat16) with_q((__nv_bfloat16*)nullptr);
+  else with_q((float*)nullptr);
 }
 
 }  // namespace mb

@@ -275,7 +275,7 @@ def kv_compact(k_caches, v_caches, tables, lens, out=None):
         out = torch.empty_like(tables)
     remap = torch.empty(pages, dtype=torch.int32, device=dev)
     live = torch.empty(1, dtype=torch.int32, device=dev)
-    ws = torch.empty(3 * pages + 1, dtype=torch.int32, device=dev)
+    ws = torch.empty(2 * pages + 1, dtype=torch.int32, device=dev)
     _C().kv_compact(k_caches, v_caches, tables, lens, out, remap, live, ws)
     return out, remap, live
 
