@@ -158,6 +158,14 @@ class EnginePlugin(TextModelPluginInterface):
         out = self.generate_ids([ids], max_new_tokens, **kwargs)[0]
         return self.detokenize(out)
 
+    def generate_samples(self, prompt: str, n: int, max_new_tokens: int = 512, **kwargs) -> List[str]:
+        """``n`` continuations of one prompt, which is computed once (``LLMEngine.generate_parallel``)."""
+        if self.engine is None:
+            self.load_model()
+        ids = self.tokenize(prompt) or [0]
+        outs = self.engine.generate_parallel([ids], n, self._params(max_new_tokens, **kwargs))[0]
+        return [self.detokenize(o) for o in outs]
+
     # ------------------------------------------------------------------ chat / code
     def format_chat(self, messages: List[Dict[str, str]], enable_thinking: Optional[bool] = None) -> str:
         """The model's chat prompt for ``messages`` (ChatML for the Qwen3 family)."""

@@ -85,10 +85,13 @@ def cmd_run(args) -> int:
         return 1
     p = pm.get_plugin(args.model)
     t0 = time.perf_counter()
-    out = p.generate_text(args.prompt, max_new_tokens=args.max_new_tokens, temperature=args.temperature)
+    if args.n > 1:
+        outs = p.generate_samples(args.prompt, args.n, max_new_tokens=args.max_new_tokens, temperature=args.temperature)
+    else:
+        outs = [p.generate_text(args.prompt, max_new_tokens=args.max_new_tokens, temperature=args.temperature)]
     dt = time.perf_counter() - t0
-    print(out)
-    print(f"[{args.max_new_tokens} tokens in {dt:.2f} s]", file=sys.stderr)
+    print("\n---\n".join(outs))
+    print(f"[{args.max_new_tokens} tokens{f' x {args.n}' if args.n > 1 else ''} in {dt:.2f} s]", file=sys.stderr)
     return 0
 
 
@@ -280,6 +283,7 @@ def build_parser() -> argparse.ArgumentParser:
         if name == "run":
             p.add_argument("--prompt", required=True)
             p.add_argument("--temperature", type=float, default=0.0)
+            p.add_argument("--n", type=int, default=1, help="continuations of the prompt, sampled together")
         else:
             p.add_argument("--thinking", action="store_true")
         p.set_defaults(fn=fn)

@@ -26,6 +26,7 @@ class ForwardBatch:
     ctx_lens_host: List[int] = field(default_factory=list)
     attn_splits: int = 1
     inputs_embeds: Optional[torch.Tensor] = None          # [T, H] (vision tokens merged in)
+    shared_plan: Optional[object] = None                  # schedule of attn_shared: sequences in groups with a common prefix
 
     @property
     def num_seqs(self) -> int:

@@ -1,13 +1,14 @@
 """Paged KV block allocator (block size 16) and recurrent-state slot pool.
 
 A LIFO free list of physical block ids; a sequence owns the blocks listed in
-its table.  Allocation failure returns False so the scheduler can preempt
+its table, and forked sequences own the full blocks that they share together
+(a block is freed with its last owner).  Allocation failure returns False so the scheduler can preempt
 instead of crashing (the reference has no KV allocator: its caches are
 static per generate call, ``pio/models/qwen3_0_6b/architecture.py:195-201``).
 """
 from __future__ import annotations
 
-from typing import List
+from typing import Dict, List, Optional, Tuple
 
 from .sequence import Sequence
 
@@ -19,6 +20,7 @@ class BlockManager:
         self.free: List[int] = list(range(num_blocks - 1, -1, -1))
         self.free_slots: List[int] = list(range(max_seqs - 1, -1, -1))
         self.max_seqs = max_seqs
+        self.owners: Dict[int, int] = {}     # blocks of forked sequences with more than one owner
 
     @property
     def num_free(self) -> int:
@@ -42,13 +44,54 @@ class BlockManager:
             seq.state_slot = self.free_slots.pop()
         return True
 
+    def _disown(self, block: int) -> bool:
+        """One owner less; True when it was the last one."""
+        n = self.owners.get(block, 1) - 1
+        if n > 1:
+            self.owners[block] = n
+        else:
+            self.owners.pop(block, None)
+        return n == 0
+
     def release(self, seq: Sequence) -> None:
-        self.free.extend(reversed(seq.blocks))
+        self.free.extend(b for b in reversed(seq.blocks) if self._disown(b))
         seq.blocks = []
         if seq.state_slot >= 0:
             self.free_slots.append(seq.state_slot)
             seq.state_slot = -1
         seq.num_cached = 0
+
+    def _take(self) -> int:
+        return self.free.pop()
+
+    def fork(self, parent: Sequence, child: Sequence) -> Optional[List[Tuple[int, int]]]:
+        """``child`` (without blocks) continues ``parent``'s cached tokens: it shares the full blocks, and the partly
+        filled last one is to be copied.  Returns the (source, target) pairs of that copy, or None where no block or
+        slot is free.  Full blocks are never written again, so sharing needs no further care."""
+        full, part = divmod(parent.num_cached, self.block_size)
+        if child.blocks or (part and self.num_free < 1) or (child.state_slot < 0 and not self.free_slots):
+            return None
+        child.blocks = list(parent.blocks[:full])
+        for b in child.blocks:
+            self._share(b)
+        pairs = []
+        if part:
+            child.blocks.append(self._take())
+            pairs.append((parent.blocks[full], child.blocks[full]))
+        if child.state_slot < 0:
+            child.state_slot = self.free_slots.pop()
+        child.num_cached = parent.num_cached
+        return pairs
+
+    def _share(self, block: int) -> None:
+        self.owners[block] = self.owners.get(block, 1) + 1
+
+    def moved(self, remap: List[int]) -> None:
+        """The blocks in use went from id b to remap[b] (-1: in no sequence's table); sequences' tables are rewritten by
+        the caller."""
+        self.owners = {remap[b]: n for b, n in self.owners.items()}
+        used = {r for r in remap if r >= 0}
+        self.free = [b for b in range(self.num_blocks - 1, -1, -1) if b not in used]
 
     def slot_of(self, seq: Sequence, pos: int) -> int:
         return seq.blocks[pos // self.block_size] * self.block_size + pos % self.block_size
@@ -140,11 +183,31 @@ class PrefixCachingBlockManager(BlockManager):
                 self.ref[b] -= 1
                 if self.ref[b] == 0:
                     self.lru[b] = None
-            else:
+            elif self._disown(b):
                 self.free.append(b)
         seq.blocks = []
         seq.num_cached = 0
         seq.registered = 0
+
+    def fork(self, parent: Sequence, child: Sequence):
+        pairs = super().fork(parent, child)
+        if pairs is not None:
+            child.registered = getattr(parent, "registered", 0)
+        return pairs
+
+    def _share(self, block: int) -> None:
+        if block in self.hash_of:
+            self.ref[block] += 1
+        else:
+            super()._share(block)
+
+    def moved(self, remap: List[int]) -> None:
+        """Cached blocks without users are in no table: they are given up."""
+        super().moved(remap)
+        self.hash_of = {remap[b]: h for b, h in self.hash_of.items() if remap[b] >= 0}
+        self.cache = {h: b for b, h in self.hash_of.items()}
+        self.ref = {remap[b]: n for b, n in self.ref.items() if remap[b] >= 0}
+        self.lru.clear()
 
     def release(self, seq: Sequence) -> None:
         self._drop(seq)
@@ -167,5 +230,5 @@ class PrefixCachingBlockManager(BlockManager):
                 continue                        # already shared, or the same content lives in another block
             self.cache[h] = b
             self.hash_of[b] = h
-            self.ref[b] = 1
+            self.ref[b] = self.owners.pop(b, 1)   # a forked block's owners become its users
         seq.registered = done

@@ -39,6 +39,33 @@ class KVCache:
         j = self.layer_index[i]
         return self.k[j], self.v[j]
 
+    def _ops(self):
+        if self.k[0].is_cuda:
+            from ..ops import native
+
+            return native
+        from ..ops import reference
+
+        return reference
+
+    def copy_pages(self, pairs) -> None:
+        """Copies blocks in every layer: ``pairs`` of (source, target), no target twice or also a source."""
+        pairs = list(pairs)
+        if not pairs or not self.k:
+            return
+        src, dst = torch.tensor(pairs, dtype=torch.int32).t().contiguous().to(self.k[0].device)
+        self._ops().kv_copy_pages(self.k, self.v, src, dst)
+
+    def compact(self, tables):
+        """Moves the blocks that ``tables`` (lists of block ids) refer to to the lowest ids in every layer.  Returns the
+        new id of every block (-1: in no table) and the number of blocks in use."""
+        width = max([1] + [len(t) for t in tables])
+        rows = torch.tensor([t + [0] * (width - len(t)) for t in tables], dtype=torch.int32).view(len(tables), width)
+        lens = torch.tensor([len(t) * self.block_size for t in tables], dtype=torch.int32)
+        dev = self.k[0].device
+        _, remap, live = self._ops().kv_compact(self.k, self.v, rows.to(dev), lens.to(dev))
+        return remap.tolist(), int(live)
+
     @staticmethod
     def bytes_per_block(cfg: ModelConfig, block_size: int = 16, dtype=torch.bfloat16, num_kv_heads: int = None) -> int:
         n_attn = sum(1 for i in range(cfg.num_hidden_layers) if cfg.layer_type(i) == "full_attention")

@@ -479,6 +479,25 @@ class LLMEngine:
             out.append(s.output)
         return out
 
+    def generate_parallel(self, prompts: List[Seq[int]], n: int, params: Optional[SamplingParams] = None,
+                          drafts: int = 4) -> List[List[List[int]]]:
+        """``n`` continuations of each prompt, computed once and forked; see ``engine.parallel_sampling``."""
+        from .parallel_sampling import ParallelSampler
+
+        return ParallelSampler(self, drafts=drafts).generate(prompts, n, params)
+
+    def compact_kv(self, extra: Optional[List[Sequence]] = None) -> int:
+        """Between steps: moves the KV blocks of all sequences (those of the scheduler and ``extra``) to the lowest ids
+        of the pool, so that everything past the returned number of blocks is free in one piece.  Prefix-cached blocks
+        without a user are given up."""
+        seqs = {id(s): s for s in [*self.scheduler.running, *self.scheduler.waiting, *(extra or [])] if s.blocks}
+        remap, live = self.kv.compact([s.blocks for s in seqs.values()])
+        self.blocks.moved(remap[:self.blocks.num_blocks])
+        for s in seqs.values():
+            s.blocks = [remap[b] for b in s.blocks]
+            self.runner.forget_table(s)
+        return live
+
     def stats(self) -> Dict[str, float]:
         return {"free_blocks": self.blocks.num_free, "running": len(self.scheduler.running),
                 "waiting": len(self.scheduler.waiting), "preempted": self.scheduler.num_preempted,

@@ -1,0 +1,213 @@
+"""Several continuations of each prompt, sampled together.
+
+1. each prompt is prefilled once;
+2. it is forked into n sequences: their block tables share the prompt's full blocks, the partly filled last block is
+   copied for each (one page-copy launch over all layers);
+3. a step runs every sequence's last token and its n-gram drafts (``speculative.ngram_propose``) in one forward, whose
+   attention reads the blocks of a common prompt once for all of its sequences (``attn_shared``);
+4. the drafts are verified against the target's probabilities with given random numbers (``verify_sampled``): the
+   emitted tokens follow the same distribution as sampling one token after another, greedy requests give the greedy
+   tokens.  KV entries of refused drafts are overwritten later.
+
+On other backends than the native one the same steps run on the plain restatements of the operators.  Attention-only
+models in a single process, as for n-gram speculation: recurrent state can neither be shared nor rolled back.
+"""
+from __future__ import annotations
+
+import time
+from typing import List, Optional, Sequence as Seq
+
+import numpy as np
+import torch
+
+from .batch import ForwardBatch
+from .sampler import filter_logits
+from .sequence import SamplingParams, Sequence, SeqStatus
+from .speculative import SpecStats, ngram_propose
+
+
+class ParallelSampler:
+    def __init__(self, engine, drafts: int = 4, ngram_max: int = 3, ngram_min: int = 1):
+        if engine.runner.states is not None:
+            raise ValueError("parallel sampling needs attention-only models (recurrent state cannot roll back)")
+        if getattr(engine, "expert_parallel", False) or getattr(engine, "tensor_parallel", False):
+            raise ValueError("parallel sampling runs in a single process")
+        self.eng, self.k, self.nmax, self.nmin = engine, drafts, ngram_max, ngram_min
+        self.native = getattr(engine.backend, "N", None) is not None and engine.device.type == "cuda"
+        # on tensor cores a query group's head dim is 64, 128 or 256; elsewhere the prefill path serves
+        self.shared = self.native and engine.cfg.head_dim in (64, 128, 256)
+        self.stats = SpecStats()
+        self.gen: Optional[torch.Generator] = None
+
+    # ------------------------------------------------------------------ random numbers
+    def _seed(self, params: SamplingParams) -> None:
+        self.gen = torch.Generator(device=self.eng.device)
+        if params.seed is not None:
+            self.gen.manual_seed(params.seed)
+        else:
+            self.gen.seed()
+
+    # ------------------------------------------------------------------ verification
+    def _verify(self, logits: torch.Tensor, counts: List[int], drafts: List[List[int]], seqs: List[Sequence]):
+        """logits [sum(counts + 1), V] -> (accepted drafts, next token) of each sequence."""
+        dev, B, K = logits.device, len(counts), max([1] + counts)
+        ps = [s.params for s in seqs]
+        heat = [max(p.temperature, 0.0) for p in ps]
+        if any(t > 0 and (p.top_k > 0 or p.top_p < 1) for t, p in zip(heat, ps)):
+            rows = [i for i, c in enumerate(counts) for _ in range(c + 1)]
+            f = filter_logits(logits.float(), torch.tensor([heat[i] or 1.0 for i in rows], device=dev),
+                              torch.tensor([ps[i].top_k for i in rows], device=dev),
+                              torch.tensor([ps[i].top_p for i in rows], device=dev))
+            sampled = torch.tensor([heat[i] > 0 for i in rows], device=dev)
+            logits = torch.where(sampled[:, None], f, logits.float())   # filtered logits are already divided
+            heat = [1.0 if t > 0 else 0.0 for t in heat]
+        cu = torch.tensor(np.cumsum([0] + [c + 1 for c in counts]), dtype=torch.int32).to(dev)
+        ids = torch.tensor([d + [0] * (K - len(d)) for d in drafts], dtype=torch.long).view(B, K).to(dev)
+        uniforms = torch.rand(B, K, device=dev, generator=self.gen)
+        noise = torch.empty(B, logits.shape[1], device=dev).exponential_(generator=self.gen)
+        if self.native:
+            ops = self.eng.backend.N
+        else:
+            from ..ops import reference as ops
+        acc, tok, _ = ops.verify_sampled(logits.contiguous(), cu, ids, uniforms, noise,
+                                         torch.tensor(heat, dtype=torch.float32).to(dev))
+        acc, tok = torch.stack([acc.long(), tok]).tolist()
+        if min(tok, default=0) < 0:
+            raise RuntimeError("a row of logits has no finite entry")
+        return acc, tok
+
+    # ------------------------------------------------------------------ one step
+    def _forward(self, seqs: List[Sequence], drafts: List[List[int]], groups: List[int], shared: List[int]):
+        """Logits of every sequence's last token and drafts; ``groups``: sequences of each prompt (in order) and
+        ``shared``: tokens whose blocks they have in common."""
+        r = self.eng.runner
+        bs, dev = r.blocks.block_size, r.device
+        ids, pos, slots, ctx, qlens = [], [], [], [], []
+        bt = np.zeros((len(seqs), r.max_blocks), dtype=np.int32)
+        for i, (s, d) in enumerate(zip(seqs, drafts)):
+            start = s.length - 1                     # the last emitted token is not cached yet
+            p = np.arange(start, start + 1 + len(d))
+            ids += [s.last_token] + d
+            pos.append(p)
+            slots.append(np.asarray(s.blocks)[p // bs] * bs + p % bs)
+            ctx.append(start + 1 + len(d))
+            qlens.append(1 + len(d))
+            bt[i, :len(s.blocks)] = s.blocks
+
+        def up(x, dtype=torch.int32):
+            return torch.as_tensor(np.asarray(x)).to(dtype).to(dev)
+
+        T = len(ids)
+        fb = ForwardBatch(input_ids=up(ids, torch.long), positions=up(np.concatenate(pos)),
+                          slot_mapping=up(np.concatenate(slots)), block_tables=torch.from_numpy(bt).to(dev),
+                          ctx_lens=up(ctx), logits_idx=torch.arange(T, device=dev),
+                          state_slots=up([s.state_slot for s in seqs], torch.long), is_decode=False, query_lens=qlens,
+                          ctx_lens_host=ctx)
+        if self.shared:  # one schedule for all layers of the step
+            m = r.model
+            fb.shared_plan = self.eng.backend.N.attn_shared_plan(
+                fb.block_tables, fb.ctx_lens, up(np.cumsum([0] + groups)), up(shared), T, m.Hq, m.Hkv,
+                self.eng.cfg.head_dim, cu_q=up(np.cumsum([0] + qlens)))
+        return r.model.logits(r.model.forward(fb, r.kv, r.states))
+
+    def _step(self, running: List[List[Sequence]], shared: List[int]) -> None:
+        eng = self.eng
+        seqs = [s for g in running for s in g]
+        drafts = []
+        for s in seqs:
+            room = min(self.k, s.params.max_new_tokens - len(s.output) - 1,
+                       eng.runner.max_blocks * eng.blocks.block_size - s.length)
+            d = ngram_propose(s.all_tokens, room, self.nmax, self.nmin) if room > 0 else []
+            if d and not eng.blocks.allocate(s, s.length + len(d)):
+                d = []
+            if not eng.blocks.allocate(s, s.length):
+                raise RuntimeError("KV cache exhausted during parallel sampling")
+            drafts.append(d)
+        logits = self._forward(seqs, drafts, [len(g) for g in running], shared)
+        acc, tok = self._verify(logits, [len(d) for d in drafts], drafts, seqs)
+        self.stats.steps += 1
+        for s, d, a, t in zip(seqs, drafts, acc, tok):
+            s.num_cached = s.length + a              # the last token and the accepted drafts
+            self.stats.drafted += len(d)
+            self.stats.accepted += a
+            self._emit(s, d[:a] + [t])
+
+    def _emit(self, s: Sequence, tokens: List[int]) -> None:
+        n = 0
+        for t in tokens:
+            s.output.append(int(t))
+            n += 1
+            if s.finished_by(int(t)):
+                s.status, s.t_finish = SeqStatus.FINISHED, time.perf_counter()
+                self.eng.blocks.release(s)
+                break
+        self.stats.emitted += n
+        self.stats.per_step.append(n)
+
+    # ------------------------------------------------------------------ a wave of prompts
+    def _wave(self, prompts: List[Seq[int]], n: int, params: SamplingParams) -> List[List[List[int]]]:
+        eng, bs = self.eng, self.eng.blocks.block_size
+        parents = [Sequence(prompt=[int(t) for t in p], params=params) for p in prompts]
+        children = [[Sequence(prompt=list(p.prompt), params=params) for _ in range(n)] for p in parents]
+        try:
+            rows, at = [], 0
+            while at < len(parents):  # the prompts, as many at a time as a prefill step takes
+                end, tokens = at, 0
+                while end < len(parents) and (end == at or tokens + parents[end].length <= eng.scheduler.max_prefill_tokens):
+                    if not eng.blocks.allocate(parents[end], parents[end].length):
+                        raise RuntimeError("KV cache exhausted during parallel sampling")
+                    tokens += parents[end].length - parents[end].num_cached
+                    end += 1
+                part = parents[at:end]
+                rows.append(eng.runner.prefill(part, [p.length - p.num_cached for p in part], return_logits=True))
+                at = end
+            logits = torch.cat(rows)
+            pairs = []
+            for p, cs in zip(parents, children):
+                if eng.prefix_caching:
+                    eng.blocks.register(p)
+                for c in cs:
+                    c.status = SeqStatus.RUNNING
+                    got = eng.blocks.fork(p, c)
+                    if got is None:
+                        raise RuntimeError("KV cache exhausted during parallel sampling")
+                    pairs += got
+            eng.kv.copy_pages(pairs)
+            for p in parents:
+                eng.blocks.release(p)
+            every = [c for cs in children for c in cs]
+            _, tok = self._verify(logits.repeat_interleave(n, 0), [0] * len(every), [[] for _ in every], every)
+            for c, t in zip(every, tok):
+                self._emit(c, [t])
+            most = len(every)
+            while True:
+                running = [[c for c in cs if c.status == SeqStatus.RUNNING] for cs in children]
+                shared = [len(p.prompt) // bs * bs for p, g in zip(parents, running) if g]
+                running = [g for g in running if g]
+                left = sum(len(g) for g in running)
+                if not left:
+                    break
+                if 2 * left <= most:  # many have finished: their blocks lie between those that stay
+                    eng.compact_kv([c for g in running for c in g])
+                    most = left
+                self._step(running, shared)
+            return [[c.output for c in cs] for cs in children]
+        finally:
+            for s in [*parents, *(c for cs in children for c in cs)]:
+                if s.blocks or s.state_slot >= 0:
+                    eng.blocks.release(s)
+
+    def generate(self, prompts: List[Seq[int]], n: int, params: Optional[SamplingParams] = None) -> List[List[List[int]]]:
+        """``n`` continuations of each prompt.  At most the engine's batch of sequences runs at a time."""
+        params = params or SamplingParams()
+        room = self.eng.blocks.max_seqs // (n + 1)   # a slot for each prompt while it is forked
+        if n < 1 or room < 1:
+            raise ValueError(f"n = {n}: between 1 and {self.eng.blocks.max_seqs - 1} (the engine's batch less the prompt's)")
+        if any(len(p) < 1 or len(p) + params.max_new_tokens > self.eng.runner.max_blocks * self.eng.blocks.block_size
+               for p in prompts):
+            raise ValueError("a prompt is empty or does not fit the model length with its new tokens")
+        self._seed(params)
+        out: List[List[List[int]]] = []
+        for i in range(0, len(prompts), room):
+            out += self._wave(prompts[i:i + room], n, params)
+        return out

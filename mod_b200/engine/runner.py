@@ -108,6 +108,10 @@ class ModelRunner:
             return self.sampler(self.model.logits(h), seqs)
         return self.model.sample_greedy(h)
 
+    def forget_table(self, seq: Sequence) -> None:
+        """The sequence's blocks have moved: its row of the step buffers is written anew."""
+        self._gen[seq.req_id] = self._gen.get(seq.req_id, 0) + 1
+
     # ------------------------------------------------------------------ decode
     def _decode_body(self, B: int) -> torch.Tensor:
         h = self.model.forward(self._fb_decode(B), self.kv, self.states)

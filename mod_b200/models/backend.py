@@ -239,6 +239,10 @@ class NativeBackend:
         cu_q = torch.tensor(cu, dtype=torch.int32).to(q.device, non_blocking=True)
         return self.N.attn_prefill_tc(q, k_cache, v_cache, fb.block_tables, cu_q, fb.ctx_lens, max(ql))
 
+    def attn_shared(self, q, k_cache, v_cache, fb):
+        """A step whose sequences come in groups with a common prefix, by its schedule ``fb.shared_plan``."""
+        return self.N.attn_shared(q, k_cache, v_cache, fb.block_tables, fb.shared_plan)
+
     def moe(self, x, mo, top_k, renorm, inter, residual=None):
         N = self.N
         T, H = x.shape

@@ -58,7 +58,9 @@ class DecoderLM:
             qkv = be.linear(x, aw.qkv, bias=aw.qkv_bias)
             be.rope_qknorm(qkv, aw.q_norm, aw.k_norm, fb.positions, self.inv_freq, fb.slot_mapping, q, kc, vc, Hq,
                            Hkv, D, cfg.rotary_dim, cfg.rms_norm_eps)
-        if hasattr(be, "attn_paged"):
+        if fb.shared_plan is not None:
+            o = be.attn_shared(q, kc, vc, fb)
+        elif hasattr(be, "attn_paged"):
             o = be.attn_paged(q, kc, vc, fb)
         elif fb.is_decode:
             o = be.attn_decode(q, kc, vc, fb.block_tables, fb.ctx_lens, fb.attn_splits)
