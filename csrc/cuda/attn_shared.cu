@@ -12,27 +12,37 @@
 // of its rows (a row is a query token and a query head of one KV head's group), each sequence's own tokens for its own
 // rows, and long key ranges are cut anywhere.
 //
-// Work: a unit is up to 256 rows that read one key range for one KV head: a group's prefix (256 rows: two 128-row
-// tiles against the same key tiles) or a sequence's own tokens (128 rows).  The plan kernel lists the units of a step
-// with their costs and cuts the list into one equal share for every SM, at key-tile boundaries, so that the few long
-// prefixes and the many short tails of a batch fill the GPU alike.  Units that a cut divides, and rows that have a
-// prefix and a tail, leave (o, m, l) partials in fp32 which the merge kernel joins; the others are written at once.
+// Three launches after the step's plan: own tokens of few rows (lean kernel), the other units (attention kernel), join
+// (merge kernel).
+//
+// Work of the attention kernel: a unit is up to 256 rows that read one key range for one KV head: a group's prefix (256
+// rows: two 128-row tiles against the same key tiles) or the own tokens of a sequence with many query rows (128 rows).
+// The plan kernel lists the units of a step with their costs and cuts the list into equal shares, one for every SM, at
+// key-tile boundaries, so that long and short prefixes fill the GPU alike.  Units that a cut divides, and rows that have
+// a prefix and a tail, leave (o, m, l) partials in fp32 which the merge kernel joins; the others are written at once.
 //
 // The attention kernel is one persistent CTA per SM:
 //   TMA warp   : key tiles (K, then V) of 64 tokens, one copy per page, into a ring of slots
 //   Q warp     : the rows of the next pieces into two tile buffers (128-byte swizzle; by cp.async where the heads of a
 //                group do not divide a tile)
-//   MMA warp   : S = Q.K^T (fp32 in TMEM), O += P.V with P read from TMEM (it overwrites S
-//                as bf16; 32 columns of S hold 32 keys' P and, where it has two terms, the second one's)
-//   2 x 8 warps: softmax of one 128-row tile each, a row a thread; a row's O is rescaled only where its running
+//   2 MMA warps: S = Q.K^T (fp32 in TMEM), O += P.V with P read from TMEM, where it overwrites S as bf16: 32 columns of S
+//                hold 32 keys' P
+//   2 x 4 warps: softmax of one 128-row tile each, a row a thread; a row's O is rescaled only where its running
 //                maximum has grown by more than 2^8 (P stays below 256, so bf16 and fp32 lose nothing)
 // The two tiles are independent pipelines that share the tensor cores, and each has two S: while the softmax of one
-// runs, the products of the other are done.  A piece of one tile only lets its even and odd key tiles take the two pipelines and joins their halves in TMEM.
-// At D = 256 TMEM holds one pipeline.  Sums, maxima and O stay in fp32.  For one-tile pieces, which wait for memory and
-// not for the tensor cores, P enters the second product as two bf16 terms (16 bits of it, over S's whole columns), so
-// that few keys leave no more than the output's rounding; two-tile pieces round P to bf16, whose errors of 2^-9 average
-// out over the many keys of a prefix.  Token slots past the context may hold anything: their scores are
-// masked by selection and their V columns are zeroed in shared memory.  Every wait is bounded.
+// runs, the products of the other are done.  A piece of one tile only lets its even and odd key tiles take the two
+// pipelines and joins their halves in TMEM.  At D = 256 TMEM holds one pipeline.
+//
+// Sums, maxima and O are in fp32.  P enters the second product as two bf16 terms (16 bits of it): one term alone makes the
+// whole result's error 1.4 times that of its final rounding, two cost 1 to 4% of the time (132 -> 133 us on 32768 shared
+// tokens under 128 sequences, 33 -> 35 us on 8192 under 64), since the softmax and not the tensor cores bounds a tile.
+// Token slots past the context may hold anything: their scores are masked by selection and their V columns are zeroed
+// in shared memory.  Every wait is bounded.
+//
+// Measured on one B200 (whole call in a CUDA graph): 32 heads on 4 KV heads, 32768 shared tokens under 128 sequences with
+// up to 1024 own: 133 us, 530 TFLOP/s; bound by the softmax of a 64-key tile (about 1450 clocks in each of two warps an
+// SM quarter, of 1900 a step).  2048 shared under 64 with up to 512 own: 30 us, of which about 12 the own tokens, 11 the
+// prefix (a start of 4500 clocks and 9000 clocks to write 256 partial rows an SM around one step) and the rest the join.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <torch/extension.h>
@@ -53,12 +63,17 @@ constexpr int kWideRows = 256;    // rows of a prefix unit at D <= 128 (two tile
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 64;
 constexpr int kNoLimit = 1 << 29;
-constexpr int kLeanRows = 64;     // sequences of up to this many rows take the lean kernel for their own tokens (D <= 128)
+// Own tokens of up to kLeanRows rows a sequence take the lean kernel (D <= 128): 20 rows of drafts 34 us there, 36 us as
+// units of the attention kernel.
+constexpr int kLeanRows = 64;
 constexpr int kLeanWarps = 16;    // lean pieces aimed at, for each SM
-constexpr int kSplitKeys = 4096;  // prefixes below this enter the second product as two bf16 terms as well
+constexpr int kLeanPages = 8;     // least pages of a piece (4 instead: -2 us on drafts, +2 us on 8 x 16 samples)
 
-// Costs: a tile of keys against one and against two tiles of rows, and a unit's start and end.
+// Costs: a tile of keys against one and against two tiles of rows, and a unit's start and end.  A share costs its partial
+// rows, written and read again, so none is cheaper than kCostShare (measured 1 / 8 / 12 / 24 / 40: 16 sequences on 8192
+// tokens 27 / 25 / 23 / 25 / 32 us, 64 on 2048 31 / 30 / 33 / 36 / 43 us).
 constexpr int kCostNarrow = 2, kCostWide = 3, kCostUnit = 8;
+constexpr int kCostShare = 8;
 
 struct Unit {
   int row0;      // first row, in (token, head of the group) order
@@ -162,7 +177,7 @@ __device__ __forceinline__ int last_le(const int* a, int n, int x) {
   return lo;
 }
 
-// One CTA; a few microseconds a step, against tens of attention launches that use its result.
+// One CTA, once a step; every layer's launches use its result.
 __global__ void __launch_bounds__(kPlanThreads)
     attn_shared_plan_kernel(const int* __restrict__ ctx_lens, const int* __restrict__ group_offs,
                             const int* __restrict__ shared_lens, const int* __restrict__ cu_q, int* plan, PlanDims d,
@@ -218,9 +233,9 @@ __global__ void __launch_bounds__(kPlanThreads)
     if (le[b]) atomicAdd(&lean_pages, le[b] * ((c - p + 15) / 16));
   }
   __syncthreads();
-  // pages of a lean piece: as many pieces as the warps that run them, but no less than 8 pages (4 KB of K and of V each)
+  // pages of a lean piece: as many pieces as the warps that run them, but no less than kLeanPages
   const int64_t page_work = (int64_t)lean_pages * d.Hkv;
-  const int chunk = (int)max((int64_t)8, (page_work + d.shares * kLeanWarps - 1) / (d.shares * kLeanWarps));
+  const int chunk = (int)max((int64_t)kLeanPages, (page_work + d.shares * kLeanWarps - 1) / (d.shares * kLeanWarps));
   for (int b = tid; b < d.B; b += kPlanThreads) {
     const int g = group_of(b), pages = (ctx_of(b) - (g >= 0 ? pre[g] : 0) + 15) / 16;
     const int chunks = le[b] ? (pages + chunk - 1) / chunk : 0;
@@ -290,10 +305,11 @@ __global__ void __launch_bounds__(kPlanThreads)
   __syncthreads();
   const int W0 = v.cost[n];
   const int64_t W = (int64_t)W0 * d.Hkv;
+  const int shares = (int)min((int64_t)d.shares, max((int64_t)1, W / kCostShare));
   for (int c = tid; c <= d.shares; c += kPlanThreads) {
     int u = n * d.Hkv, t = 0;
-    if (c < d.shares && W > 0) {
-      const int64_t target = W * c / d.shares;
+    if (c < shares && W > 0) {
+      const int64_t target = W * c / shares;
       const int hk = (int)(target / W0), rem = (int)(target % W0);
       const int u0 = last_le(v.cost, n, rem);
       const Unit& e = reinterpret_cast<const Unit*>(v.units)[u0];
@@ -459,7 +475,7 @@ struct Walk {
   int n, u, t, u_end, t_end;
   Unit e;
   int hk, u0, t0, t1;
-  bool wide, split;  // two tiles against the same keys; P as two bf16 terms
+  bool wide;  // two tiles against the same keys
   __device__ Walk(const PlanView& v, int share) {
     units = reinterpret_cast<const Unit*>(v.units);
     n = v.hdr[0];
@@ -485,7 +501,6 @@ struct Walk {
       t = 0;
       if (t1 > t0) {
         wide = e.rows > kTileRows;
-        split = !wide || e.key_end < kSplitKeys;
         return true;
       }
     }
@@ -607,16 +622,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 #pragma unroll
           for (int kb = 0; kb < C::kBlocks; ++kb)
             mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8, vd + kb * (D * 32 / 16), idesc_o, kb ? 1 : acc);
-          if (w.split) {
 #pragma unroll
-            for (int kb = 0; kb < C::kBlocks; ++kb)
-              mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8 + 16, vd + kb * (D * 32 / 16), idesc_o, 1);
-          }
+          for (int kb = 0; kb < C::kBlocks; ++kb)
+            mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8 + 16, vd + kb * (D * 32 / 16), idesc_o, 1);
         } else {
 #pragma unroll 1
           for (int kb = 0; kb < blocks; ++kb) {
             mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8, vd + kb * (D * 32 / 16), idesc_o, kb ? 1 : acc);
-            if (w.split) mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8 + 16, vd + kb * (D * 32 / 16), idesc_o, 1);
+            mma_ts(o, w0 + (kb >> 1) * 32 + (kb & 1) * 8 + 16, vd + kb * (D * 32 / 16), idesc_o, 1);
           }
         }
         tc_commit(&empty[slot]);
@@ -789,7 +802,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     bool ok = true;
     while (ok && w.next()) {
       const int nt = w.t1 - w.t0;
-      const bool wide = w.wide, split = w.split;
+      const bool wide = w.wide;
       const int rows = w.e.rows - (wide ? p * kTileRows : 0);  // rows of this tile (may exceed 128)
       const bool live = (row & ~31) < rows;                     // some row of this warp is one
       const int key0 = w.e.key0 + w.t0 * KT;                    // of the piece
@@ -860,13 +873,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
               s[c + e + 1] = __float_as_uint(x.y);
             }
             tmem_st16(tS + c, pk);
-            if (split) {  // what the rounding left, as a second product's weights, over the other 16
+            // what the rounding left, as a second product's weights, over the other 16
 #pragma unroll
-              for (int e = 0; e < 32; e += 2)
-                pk[e >> 1] = pack_bf16(__uint_as_float(s[c + e]) - __uint_as_float(pk[e >> 1] << 16),
-                                       __uint_as_float(s[c + e + 1]) - __uint_as_float(pk[e >> 1] & 0xffff0000u));
-              tmem_st16(tS + c + 16, pk);
-            }
+            for (int e = 0; e < 32; e += 2)
+              pk[e >> 1] = pack_bf16(__uint_as_float(s[c + e]) - __uint_as_float(pk[e >> 1] << 16),
+                                     __uint_as_float(s[c + e + 1]) - __uint_as_float(pk[e >> 1] & 0xffff0000u));
+            tmem_st16(tS + c + 16, pk);
           }
           l += sum.x + sum.y;
           tmem_wait_st();
@@ -991,7 +1003,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 // of the 16 x 8 x 16 products are read as the pages lie: both dimensions that are summed over are permuted for it.  Lane
 // c of a quad takes the head dims 8 (4 i + c) ... + 7 of Q and K in 16-byte loads (the same for both, so S is
 // unchanged), and the tokens 4 c ... 4 c + 3 of V's rows in 8-byte loads, which are the tokens whose S it holds.  P
-// enters the second product as two bf16 terms.
+// enters the second product as two bf16 terms.  128 sequences with up to 1024 own tokens (4 KV heads, 134 MB): about 28 us,
+// 0.73 of the measured copy rate; with one page in flight a warp 35 us.
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
   asm volatile(
@@ -1041,7 +1054,7 @@ constexpr int lean_smem() { return 4 * kLeanStages * D * 64 + 4 * kLeanStages * 
 
 template <int D>
 __global__ void __launch_bounds__(128, 2) attn_shared_lean_kernel(const __grid_constant__ LeanArgs a) {
-  constexpr int KS = D / 16, NT = D / 8, KV = D / 32;  // steps of S, column tiles of O, 16-byte loads of a K row's part
+  constexpr int NT = D / 8, KV = D / 32;  // column tiles of O, 16-byte loads of a K row's part
   constexpr int ST = kLeanStages, kPage = D * 32;       // bytes of a page of K or V of a head
   extern __shared__ __align__(128) uint8_t ring[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3, r = lane >> 2;
@@ -1208,6 +1221,9 @@ __global__ void __launch_bounds__(256)
     attn_shared_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, int* plan,
                              PlanDims d, __nv_bfloat16* __restrict__ out, int Hq, int over, int lean0) {
   constexpr int kPer = D / 32;
+  struct alignas(kPer * 4 < 16 ? kPer * 4 : 16) V {
+    float x[kPer];
+  };
   pdl_wait();
   pdl_trigger();
   const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
@@ -1265,25 +1281,29 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int e = 0; e < kPer; ++e) acc[e] *= old;
     const int cnt = min(32, total - base);
-    for (int i = 0; i < cnt; i += 4) {
-      float o[4][kPer], fi[4];
+    constexpr int kDeep = 8;
+    for (int i = 0; i < cnt; i += kDeep) {
+      V o[kDeep];
+      float fi[kDeep];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kDeep; ++k) {
         fi[k] = __shfl_sync(~0u, f, (i + k) & 31);
         const int64_t ai = __shfl_sync(~0u, at, (i + k) & 31);
         if (i + k >= cnt) fi[k] = 0.f;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) o[k][e] = fi[k] != 0.f ? part_o[ai * D + e * 32 + lane] : 0.f;
+        if (fi[k] != 0.f) o[k] = *reinterpret_cast<const V*>(part_o + ai * D + lane * kPer);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < kDeep; ++k)
+        if (fi[k] != 0.f) {  // the same for all lanes
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] += o[k][e] * fi[k];
+          for (int e = 0; e < kPer; ++e) acc[e] += o[k].x[e] * fi[k];
+        }
     }
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(out + (size_t)row * D + lane * kPer);
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) out[(size_t)row * D + e * 32 + lane] = __float2bfloat16(acc[e] * inv);
+  for (int e = 0; e < kPer; e += 2) dst[e / 2] = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
 }
 
 int sm_count(int device) {

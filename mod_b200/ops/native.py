@@ -215,7 +215,7 @@ def verify_tokens(draft, target, out=None):
 class SharedPlan:
     """Schedule of :func:`attn_shared` for one step's lengths (made by :func:`attn_shared_plan`)."""
 
-    __slots__ = ("tokens", "heads", "kv_heads", "head_dim", "table_shape", "groups", "buf", "ws_elems")
+    __slots__ = ("q_shape", "kv_heads", "table_shape", "groups", "buf", "ws_elems")
 
 
 def attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, tokens: int, heads: int, kv_heads: int,
@@ -235,8 +235,8 @@ def attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, tokens: in
     p = SharedPlan() if plan is None else plan
     if plan is None:
         p.buf = torch.empty(n, dtype=torch.int32, device=block_tables.device)
-    p.tokens, p.heads, p.kv_heads, p.head_dim = tokens, heads, kv_heads, head_dim
-    p.table_shape, p.groups, p.ws_elems = tuple(block_tables.shape), G, ws
+    p.q_shape, p.kv_heads, p.table_shape = torch.Size((tokens, heads, head_dim)), kv_heads, block_tables.shape
+    p.groups, p.ws_elems = G, ws
     _C().attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, cu_q, tokens, heads, kv_heads, head_dim,
                           p.buf)
     return p
@@ -246,8 +246,7 @@ def attn_shared(q, k_cache, v_cache, block_tables, plan: SharedPlan, out=None, s
     """Attention of a step's query tokens q [T, Hq, D] (D = 64, 128 or 256) over the paged cache, for batches whose
     sequences come in groups that share a prefix's pages; query i of a sequence's nq sees its first
     ctx - nq + i + 1 tokens.  Rows that see no token are zero.  ``plan``: from :func:`attn_shared_plan`."""
-    if tuple(q.shape) != (plan.tokens, plan.heads, plan.head_dim) or k_cache.shape[1] != plan.kv_heads or \
-            tuple(block_tables.shape) != plan.table_shape:
+    if q.shape != plan.q_shape or k_cache.shape[1] != plan.kv_heads or block_tables.shape != plan.table_shape:
         raise ValueError("attn_shared: the plan was made for other shapes")
     if out is None:
         out = torch.empty_like(q)
