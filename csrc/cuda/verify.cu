@@ -19,6 +19,10 @@
 // upper bound with the id, the second largest, and the largest lower bound.  An id below its part's largest lower bound
 // is out, so that one or two are left, and only those are computed with the correctly rounded divisions and the full
 // exponential that the outcome is defined by: three divisions for each id take longer than reading it.  Sums are in fp32.
+//
+// Measured on one B200: 64 sequences with 0 to 4 drafts, 151936 ids, bf16: 21 us for 58 MB of logits and 20 us for the
+// draws (39 MB of noise), both bound by their instructions (14 a logit in the first); 24 sequences with a draft model's
+// probabilities in fp32 13 + 17 us; one sequence 15 us, a chain of dependent loads.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
