@@ -204,6 +204,11 @@ __global__ void __launch_bounds__(kPlanThreads)
   }
   for (int i = tid; i <= d.B; i += kPlanThreads) cu[i] = cu_q ? min(max(cu_q[i], 0), d.T) : i;
   __syncthreads();
+  // What follows searches both: offsets that descend make a plan of nothing (every row is written as zeros).
+  bool bad = false;
+  for (int i = tid; i < d.G; i += kPlanThreads) bad |= offs[i + 1] < offs[i];
+  for (int i = tid; i < d.B; i += kPlanThreads) bad |= cu[i + 1] < cu[i];
+  bad = __syncthreads_or(bad);
   auto group_of = [&](int b) {
     const int g = last_le(offs, d.G + 1, b);
     return g >= 0 && g < d.G ? g : -1;
@@ -221,7 +226,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   for (int g = tid; g < d.G; g += kPlanThreads) {
     const int s0 = offs[g], s1 = offs[g + 1];
     if (s1 - s0 < 2 || lead[g] == INT_MAX) pre[g] = 0;  // nobody to share with: the sequence's own unit takes it all
-    const int rows = s1 > s0 ? (cu[s1] - cu[s0]) * d.Gq : 0;
+    const int rows = bad ? 0 : (cu[s1] - cu[s0]) * d.Gq;
     gu[g] = pre[g] > 0 ? (rows + d.wide_rows - 1) / d.wide_rows : 0;
   }
   __syncthreads();
@@ -249,7 +254,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   int n_lean = le[d.B];
   const int nG = gu[d.G];
   int n = nG + su[d.B];
-  if (n > d.max_units || n_lean > d.max_pieces) {  // only where groups overlap or cu_q descends
+  if (bad || n > d.max_units || n_lean > d.max_pieces) {
     if (tid == 0) set_status(status, kErrBounds);
     n = n_lean = 0;
   }
@@ -297,7 +302,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   }
   __syncthreads();
   block_scan(v.cost, n, sh);
-  block_scan(v.rowcum, n, sh);  // its total falls into hdr-sized slack behind the array
+  block_scan(v.rowcum, n, sh);  // its total falls into the slack behind the array
   for (int i = tid; i < n * d.Hkv; i += kPlanThreads) {
     v.inside[2 * i] = INT_MAX;
     v.inside[2 * i + 1] = 0;
@@ -793,6 +798,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         if (lane == 0) mbar_arrive(&q_full[buf]);
       }
     }
+    if (lane == 0)  // as above: the last copy into each buffer
+      for (uint32_t i = qn > NP ? qn - NP : 0; i < qn; ++i)
+        bar_wait(&q_full[i % NP], (i / NP) & 1, a.status);
   } else {
     // ---------------------------------------------------------------- softmax, a row a thread
     const int p = warp >> 2, row = tid & 127;
@@ -1385,7 +1393,7 @@ void attn_shared_plan(const at::Tensor& block_tables, const at::Tensor& ctx_lens
   const int smem = (int)(4 * (4 * G + 3 * B + 8));
   static bool attr[64] = {false};
   if (smem > 48 * 1024 && !attr[dev]) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(attn_shared_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(attn_shared_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
     attr[dev] = true;
   }
   launch_k(attn_shared_plan_kernel, 1, kPlanThreads, smem, at::cuda::getCurrentCUDAStream(), ctx_lens.data_ptr<int>(),

@@ -182,6 +182,37 @@ def test_attn_shared_prefix_longer_than_a_context(N):
     b.check(N.attn_shared(b.q, b.k, b.v, b.tables, b.plan(N)))
 
 
+def test_attn_shared_fewer_tokens_than_queries(N):
+    # query tokens that lie before the context's first token see nothing
+    b = Batch([(0, [(8, 8), (40, 40), (5, 1)])], 8, 2, 128, seed=13)
+    b.ctx = [3, 30, 5]
+    out = N.attn_shared(b.q, b.k, b.v, b.tables, b.plan(N))
+    assert (out[:5] == 0).all() and (out[8:18] == 0).all()
+    for t0, t1, c, row in ((5, 8, 3, 0), (18, 48, 30, 1), (48, 49, 5, 2)):
+        part = Batch.__new__(Batch)
+        part.q, part.k, part.v, part.tables = b.q[t0:t1], b.k, b.v, b.tables[row:row + 1]
+        part.ctx, part.cu = [c], [0, t1 - t0]
+        part.check(out[t0:t1])
+
+
+def test_attn_shared_lengths_that_do_not_fit_are_reported(N):
+    from mod_b200.ops import check_status
+
+    b = Batch([(64, seqs(5, 6, 7, 8))], 8, 2, 128, seed=14)
+    T, Hq, D = b.q.shape
+    for cu, offs in (([0, 4, 0, 4, 0], [0, 4]), ([0, 1, 2, 3, 4], [0, 4, 0, 4, 0, 4])):
+        p = N.attn_shared_plan(b.tables, ints(b.ctx), ints(offs), ints([64] * (len(offs) - 1)), T, Hq, 2, D, cu_q=ints(cu))
+        out = N.attn_shared(b.q, b.k, b.v, b.tables, p)
+        with pytest.raises(RuntimeError, match="out of bounds"):
+            check_status()
+        assert (out == 0).all()
+    # a page that there is none of counts as masked
+    b.tables[0, 4] = 10 ** 6
+    N.attn_shared(b.q, b.k, b.v, b.tables, b.plan(N))
+    with pytest.raises(RuntimeError, match="out of bounds"):
+        check_status()
+
+
 def test_attn_shared_repeats_bit_for_bit(N):
     b = Batch([(3000, seqs(*range(1, 40)))], 16, 4, 128, seed=10)
     p = b.plan(N)
