@@ -40,7 +40,7 @@
 // in shared memory.  Every wait is bounded.
 //
 // Measured on one B200 (whole call in a CUDA graph): 32 heads on 4 KV heads, 32768 shared tokens under 128 sequences with
-// up to 1024 own: 133 us, 530 TFLOP/s; bound by the softmax of a 64-key tile (about 1450 clocks in each of two warps an
+// up to 1024 own: 126 to 133 us from run to run, 540 TFLOP/s; bound by the softmax of a 64-key tile (about 1450 clocks in each of two warps an
 // SM quarter, of 1900 a step).  2048 shared under 64 with up to 512 own: 30 us, of which about 12 the own tokens, 11 the
 // prefix (a start of 4500 clocks and 9000 clocks to write 256 partial rows an SM around one step) and the rest the join.
 #include <cuda.h>
