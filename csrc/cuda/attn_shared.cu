@@ -364,7 +364,10 @@ struct Cfg {
   static constexpr int kQBytes = kTileRows * D * 2;
   static constexpr int kSoftWarps = kPipes * 4;
   static constexpr int kThreads = (kSoftWarps + kPipes + 2) * 32;
-  static constexpr int kSmem = 1024 + kPipes * kQBytes + kSlots * kSlot + kTileRows * 8 + 256;
+  static constexpr int kBars = 2 * kSlots + 9 * kPipes + 1;
+  // room to begin at a multiple of 1024 bytes, query tiles, ring, (m, l) of a tile's rows, barriers, TMEM address
+  static constexpr int kSmem = 1024 + kPipes * kQBytes + kSlots * kSlot + kTileRows * 8 + kBars * 8 + 16;
+  static_assert(kSmem <= 227 * 1024, "more shared memory than a CTA can have");
   // TMEM: two S (and P over them) of each pipeline, O behind them
   static __device__ __forceinline__ uint32_t s_col(int p, int i) { return p * 128 + i * kKeys; }
   static __device__ __forceinline__ uint32_t o_col(int p) { return 256 + p * D; }
@@ -549,7 +552,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   uint64_t* o_done = pv_done + NP;   // [NP] a piece's last one is
   uint64_t* o_free = o_done + NP;    // [NP] O has been read
   uint64_t* stat_ready = o_free + NP;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stat_ready + 1);
+  static_assert(C::kBars == 2 * NS + 9 * NP + 1, "the barriers above");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
