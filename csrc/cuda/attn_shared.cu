@@ -1396,7 +1396,7 @@ void attn_shared_plan(const at::Tensor& block_tables, const at::Tensor& ctx_lens
   TORCH_CHECK(plan.numel() >= plan_ints(d), "attn_shared_plan: plan buffer too small");
   const int smem = (int)(4 * (4 * G + 3 * B + 8));
   static bool attr[64] = {false};
-  if (smem > 48 * 1024 && !attr[dev]) {
+  if (!attr[dev]) {  // whatever this call takes: the 48 KB that need no asking count the kernel's static bytes too
     C10_CUDA_CHECK(cudaFuncSetAttribute(attn_shared_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
     attr[dev] = true;
   }

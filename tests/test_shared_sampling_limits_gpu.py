@@ -1,0 +1,61 @@
+"""The limits of the kernels behind sampling several continuations of one prompt: launch sizes at the edge of what a CTA
+may have without asking, sums past 32 bits, offsets and temperatures at the ends of their types, refused arguments."""
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from mod_b200.ops import reference as R
+from tests.test_shared_sampling_gpu import PAGE, Batch, Drafts, ints, seqs
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def N(cuda):
+    from mod_b200.ops import native
+
+    native._C()
+    return native
+
+
+@pytest.fixture(autouse=True)
+def no_status(cuda):
+    from mod_b200.ops import check_status
+
+    yield
+    torch.cuda.synchronize()
+    check_status()
+
+
+def alone(code, *args):
+    """Runs ``code`` in a process of its own, where no earlier call has asked for more shared memory."""
+    r = subprocess.run([sys.executable, "-c", code, *map(str, args)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-1500:]
+
+
+PLAN = """
+import sys, torch
+from mod_b200.ops import check_status, native as N
+B, G = map(int, sys.argv[1:])
+i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+k = torch.randn(2, 1, 16, 64, device="cuda").bfloat16()
+v = torch.randn(2, 1, 64, 16, device="cuda").bfloat16()
+q = torch.randn(B, 1, 64, device="cuda").bfloat16()
+tables, ctx = torch.ones(B, 1, dtype=torch.int32, device="cuda"), torch.ones(B, dtype=torch.int32, device="cuda")
+offs = i(list(range(B + 1))) if G == B else i([0, B])
+p = N.attn_shared_plan(tables, ctx, offs, i([0] * G), B, 1, 1, 64)
+out = N.attn_shared(q, k, v, tables, p)
+assert torch.equal(out, v[1, :, :, 0].expand(B, 1, 64))   # one key: its value
+check_status()
+"""
+
+
+# Shared memory: 4 (4 G + 3 B + 8) bytes beside 132 static ones; 48 KB is what a launch has without asking.
+@pytest.mark.parametrize("B,G", [(1749, 1749), (1750, 1750), (1754, 1754), (1755, 1755), (4082, 1), (4092, 1)])
+def test_plan_at_48_kb(B, G, cuda):
+    alone(PLAN, B, G)
