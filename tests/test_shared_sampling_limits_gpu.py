@@ -59,3 +59,24 @@ check_status()
 @pytest.mark.parametrize("B,G", [(1749, 1749), (1750, 1750), (1754, 1754), (1755, 1755), (4082, 1), (4092, 1)])
 def test_plan_at_48_kb(B, G, cuda):
     alone(PLAN, B, G)
+
+
+COMPACT = """
+import sys, torch
+from mod_b200.ops import check_status, native as N
+pages = int(sys.argv[1])
+k = [torch.zeros(pages, 1, 16, 8, dtype=torch.bfloat16, device="cuda")]
+v = [torch.zeros(pages, 1, 8, 16, dtype=torch.bfloat16, device="cuda")]
+k[0][pages - 1], v[0][pages - 1] = 1.0, 2.0
+one = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+tables, remap, live = N.kv_compact(k, v, one([[pages - 1]]), one([16]))
+assert tables.tolist() == [[0]] and int(live) == 1 and int(remap[pages - 1]) == 0
+assert (k[0][0] == 1).all() and (v[0][0] == 2).all()
+check_status()
+"""
+
+
+# A bit a page beside 128 static bytes.
+@pytest.mark.parametrize("pages", [392_192, 392_193, 393_216, 393_217])
+def test_compact_at_48_kb(pages, cuda):
+    alone(COMPACT, pages)
