@@ -191,12 +191,12 @@ __global__ void __launch_bounds__(kPlanThreads)
   int* su = gu + d.G + 1;         // [B + 1] own units
   int* le = su + d.B + 1;         // [B + 1] lean pieces
   int* cu = le + d.B + 1;         // [B + 1]
-  __shared__ int lean_pages;
+  __shared__ unsigned long long lean_pages, total_cost;  // past 32 bits with thousands of long sequences
   const PlanView v = plan_view(plan, d);
   const int tid = threadIdx.x;
   pdl_wait();
   pdl_trigger();
-  if (tid == 0) lean_pages = 0;
+  if (tid == 0) lean_pages = total_cost = 0;
   for (int i = tid; i <= d.G; i += kPlanThreads) offs[i] = min(max(group_offs[i], 0), d.B);
   for (int i = tid; i < d.G; i += kPlanThreads) {
     pre[i] = max(shared_lens[i], 0) & ~15;
@@ -235,12 +235,13 @@ __global__ void __launch_bounds__(kPlanThreads)
     const bool any = c > p && rows > 0, lean = rows <= d.lean_rows;
     su[b] = any && !lean ? (rows + kTileRows - 1) / kTileRows : 0;
     le[b] = any && lean ? (rows + 15) / 16 : 0;
-    if (le[b]) atomicAdd(&lean_pages, le[b] * ((c - p + 15) / 16));
+    if (le[b]) atomicAdd(&lean_pages, (unsigned long long)le[b] * ((c - p + 15) / 16));
   }
   __syncthreads();
   // pages of a lean piece: as many pieces as the warps that run them, but no less than kLeanPages
   const int64_t page_work = (int64_t)lean_pages * d.Hkv;
-  const int chunk = (int)max((int64_t)kLeanPages, (page_work + d.shares * kLeanWarps - 1) / (d.shares * kLeanWarps));
+  const int chunk = (int)min((int64_t)1 << 24,  // no table is wider
+                             max((int64_t)kLeanPages, (page_work + d.shares * kLeanWarps - 1) / (d.shares * kLeanWarps)));
   for (int b = tid; b < d.B; b += kPlanThreads) {
     const int g = group_of(b), pages = (ctx_of(b) - (g >= 0 ? pre[g] : 0) + 15) / 16;
     const int chunks = le[b] ? (pages + chunk - 1) / chunk : 0;
@@ -299,8 +300,13 @@ __global__ void __launch_bounds__(kPlanThreads)
     reinterpret_cast<Unit*>(v.units)[i] = u;
     v.cost[i] = u.tiles * (u.rows > kTileRows ? kCostWide : kCostNarrow) + kCostUnit;
     v.rowcum[i] = u.rows;
+    atomicAdd(&total_cost, (unsigned long long)v.cost[i]);
   }
   __syncthreads();
+  if (total_cost > INT_MAX) {  // the cuts below are searched for in 32-bit sums: a plan of nothing
+    if (tid == 0) set_status(status, kErrBounds);
+    n = n_lean = 0;
+  }
   block_scan(v.cost, n, sh);
   block_scan(v.rowcum, n, sh);  // its total falls into the slack behind the array
   for (int i = tid; i < n * d.Hkv; i += kPlanThreads) {

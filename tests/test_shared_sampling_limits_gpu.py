@@ -80,3 +80,31 @@ check_status()
 @pytest.mark.parametrize("pages", [392_192, 392_193, 393_216, 393_217])
 def test_compact_at_48_kb(pages, cuda):
     alone(COMPACT, pages)
+
+
+def plan_only(N, B, pages, heads):
+    """The schedule of B sequences of `pages` full pages, a token each, on one KV head; tables are not read for it."""
+    tables = torch.zeros(1, 1, dtype=torch.int32, device="cuda").expand(B, pages)
+    ctx = torch.full((B,), pages * PAGE, dtype=torch.int32, device="cuda")
+    return N.attn_shared_plan(tables, ctx, ints(range(B + 1)), ints([0] * B), B, heads, 1, 64)
+
+
+def test_plan_counts_pages_past_32_bits(N):
+    # 8192 sequences x 4 row tiles x 65536 pages = 2^31: a schedule like any other
+    plan_only(N, 8192, 65536, 64)
+    torch.cuda.synchronize()
+    from mod_b200.ops import check_status
+
+    check_status()
+
+
+def test_plan_costs_past_32_bits_are_reported(N):
+    # 8192 units of 131072 key tiles and more: their cost does not fit the schedule's sums, which is said
+    from mod_b200.ops import check_status
+
+    plan_only(N, 8192, 524288 + 64, 128)
+    with pytest.raises(RuntimeError, match="out of bounds"):
+        check_status()
+    plan_only(N, 4000, 524288 + 64, 128)
+    torch.cuda.synchronize()
+    check_status()
