@@ -167,8 +167,8 @@ struct VerifyArgs {
 
 // Rows of sequence b: the first one and the number of drafts, -1 where they do not lie in the logits.
 __device__ __forceinline__ int2 rows_of(const VerifyArgs& a, int b) {
-  const int r0 = a.cu[b], n = a.cu[b + 1] - r0 - 1;
-  return make_int2(r0, r0 < 0 || n < 0 || n > a.K || r0 + n >= a.num_rows ? -1 : n);
+  const int r0 = a.cu[b], r1 = a.cu[b + 1];  // compared with the ends before they are subtracted: nothing overflows
+  return make_int2(r0, r0 < 0 || r1 <= r0 || r1 > a.num_rows || r1 - r0 - 1 > a.K ? -1 : r1 - r0 - 1);
 }
 
 template <typename T>

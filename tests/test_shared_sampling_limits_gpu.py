@@ -108,3 +108,22 @@ def test_plan_costs_past_32_bits_are_reported(N):
     plan_only(N, 4000, 524288 + 64, 128)
     torch.cuda.synchronize()
     check_status()
+
+
+@pytest.mark.parametrize("cu", [[0, 3, 2 ** 31 - 1], [0, 2 ** 31 - 2, -2 ** 31 + 1], [0, -2 ** 31, 2 ** 31 - 1],
+                                [2 ** 31 - 1, -2 ** 31, 6], [0, 6, 6], [0, 0, 6]], ids=str)
+def test_verify_offsets_at_the_ends_are_reported(N, cu):
+    from mod_b200.ops import check_status
+
+    x = Drafts([2, 2], 100, [1.0], seed=3)
+    want = x.run(N)
+    x.cu = ints(cu)
+    got = x.run(N)
+    with pytest.raises(RuntimeError, match="out of bounds"):
+        check_status()
+    for b in range(2):
+        lo, hi = cu[b], cu[b + 1]
+        if (lo, hi) == (x.offs[b], x.offs[b + 1]):
+            assert all(torch.equal(g[b], w[b]) for g, w in zip(got, want))
+        else:
+            assert int(got[0][b]) == 0 and int(got[1][b]) == -1 and (got[2][b] == 0).all()
