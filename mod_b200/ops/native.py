@@ -235,10 +235,11 @@ def attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, tokens: in
     p = SharedPlan() if plan is None else plan
     if plan is None:
         p.buf = torch.empty(n, dtype=torch.int32, device=block_tables.device)
-    p.q_shape, p.kv_heads, p.table_shape = torch.Size((tokens, heads, head_dim)), kv_heads, block_tables.shape
-    p.groups, p.ws_elems = G, ws
     _C().attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, cu_q, tokens, heads, kv_heads, head_dim,
                           p.buf)
+    # only now: after a refusal the buffer still holds the earlier schedule, and the plan says so
+    p.q_shape, p.kv_heads, p.table_shape = torch.Size((tokens, heads, head_dim)), kv_heads, block_tables.shape
+    p.groups, p.ws_elems = G, ws
     return p
 
 
