@@ -1351,7 +1351,7 @@ int64_t partial_rows(const PlanDims& d, int64_t Hq) {
 
 void check_dims(const char* who, int64_t T, int64_t Hq, int64_t Hkv, int64_t D) {
   TORCH_CHECK(D == 64 || D == 128 || D == 256, who, ": head_dim must be 64, 128 or 256");
-  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && T >= 0 && T * Hq <= (int64_t)1 << 26, who, ": heads or tokens out of range");
+  TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && T >= 0 && T * Hq <= (int64_t)1 << 26, who, ": heads or tokens out of range");
 }
 
 CUtensorMap map_of(const at::Tensor& t, int rank, const cuuint64_t* dims, const cuuint64_t* strides,

@@ -127,3 +127,14 @@ def test_verify_offsets_at_the_ends_are_reported(N, cu):
             assert all(torch.equal(g[b], w[b]) for g, w in zip(got, want))
         else:
             assert int(got[0][b]) == 0 and int(got[1][b]) == -1 and (got[2][b] == 0).all()
+
+
+def test_no_heads_are_refused(N):
+    for heads in (0, -8):
+        with pytest.raises(RuntimeError, match="heads"):
+            N.attn_shared_plan(ints([[0]]), ints([1]), ints([0, 1]), ints([0]), 1, heads, 2, 64)
+    b = Batch([(0, seqs(3))], 2, 2, 64)
+    p = b.plan(N)
+    p.q_shape = torch.Size((1, 0, 64))
+    with pytest.raises(RuntimeError, match="heads"):
+        N.attn_shared(b.q[:, :0], b.k, b.v, b.tables, p)
