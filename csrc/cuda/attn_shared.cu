@@ -1400,6 +1400,7 @@ void attn_shared_plan(const at::Tensor& block_tables, const at::Tensor& ctx_lens
   const int dev = block_tables.device().index();
   const PlanDims d = plan_dims(T, B, G, Hq, Hkv, D, block_tables.size(1), dev);
   TORCH_CHECK(plan.numel() >= plan_ints(d), "attn_shared_plan: plan buffer too small");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0, "attn_shared_plan: plan must be 16-byte aligned");
   const int smem = (int)(4 * (4 * G + 3 * B + 8));
   static bool attr[64] = {false};
   if (!attr[dev]) {  // whatever this call takes: the 48 KB that need no asking count the kernel's static bytes too
@@ -1484,8 +1485,13 @@ void attn_shared(const at::Tensor& q, const at::Tensor& k_cache, const at::Tenso
   a.dims = plan_dims(T, block_tables.size(0), groups, Hq, Hkv, D, block_tables.size(1), dev);
   a.over = (int)(2 * T * Hq);
   const int64_t rows = partial_rows(a.dims, Hq);
-  TORCH_CHECK(plan.numel() >= plan_ints(a.dims) && workspace.numel() >= rows * (D + 2),
-              "attn_shared: plan or workspace too small");
+  TORCH_CHECK(plan.numel() >= plan_ints(a.dims) && workspace.numel() >= rows * (D + 2) && plan.is_contiguous() &&
+                  workspace.is_contiguous(),
+              "attn_shared: plan or workspace too small or not contiguous");
+  // records of 16 bytes, partial rows stored by 32
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(workspace.data_ptr()) % 32 == 0,
+              "attn_shared: plan must be 16-byte and workspace 32-byte aligned");
   a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
   a.tables = block_tables.data_ptr<int>();
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());

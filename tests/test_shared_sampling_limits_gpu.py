@@ -138,3 +138,25 @@ def test_no_heads_are_refused(N):
     p.q_shape = torch.Size((1, 0, 64))
     with pytest.raises(RuntimeError, match="heads"):
         N.attn_shared(b.q[:, :0], b.k, b.v, b.tables, p)
+
+
+def test_attn_shared_buffers_off_their_alignment_are_refused(N):
+    b = Batch([(40, seqs(3, 20))], 8, 2, 128)
+    p = b.plan(N)
+    C, out = N._C(), torch.empty_like(b.q)
+    ws = torch.empty(p.ws_elems + 8, dtype=torch.float32, device="cuda")
+    buf = torch.empty(p.buf.numel() + 4, dtype=torch.int32, device="cuda")
+    scale = 1 / math.sqrt(128)
+    for off in (1, 2, 4):
+        with pytest.raises(RuntimeError, match="aligned"):
+            C.attn_shared(b.q, b.k, b.v, b.tables, 1, p.buf, ws[off:], out, scale)
+    for off in (1, 2, 3):
+        with pytest.raises(RuntimeError, match="aligned"):
+            C.attn_shared(b.q, b.k, b.v, b.tables, 1, buf[off:], ws, out, scale)
+        with pytest.raises(RuntimeError, match="aligned"):
+            C.attn_shared_plan(b.tables, ints(b.ctx), ints(b.offs), ints(b.shared), None, 2, 8, 2, 128, buf[off:])
+    for plan, work in ((p.buf.repeat_interleave(2)[::2], ws), (p.buf, torch.cat([ws, ws])[::2])):
+        with pytest.raises(RuntimeError, match="contiguous"):
+            C.attn_shared(b.q, b.k, b.v, b.tables, 1, plan, work, out, scale)
+    C.attn_shared(b.q, b.k, b.v, b.tables, 1, p.buf, ws[8:], out, scale)
+    b.check(out)
