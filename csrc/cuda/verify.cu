@@ -5,7 +5,8 @@
 //   draft j is accepted where u_j q_j(d_j) < p_j(d_j);
 //   at the first refusal the next token is drawn from (p_j - q_j)+, after n acceptances from p_n,
 //   as argmax_v r(v) / noise(v) with noise ~ Exp(1) (ties: the lowest id), so emitted tokens follow p.
-// temperature <= 0: p_j is 1 at the row's largest logit (lowest id among equals).
+// temperature <= 0: p_j is 1 at the row's largest logit (lowest id among equals).  Others count as at least 2^-126 and at
+// most the largest finite number, between which 1 / temperature and what it multiplies stay numbers.
 // NaN logits count as -inf; rows without a finite or +inf logit accept nothing and give token -1.
 //
 // Bound by HBM: every logit is read once for its row's largest value and sum of exponentials, and of each sequence one
@@ -23,6 +24,8 @@
 // Measured on one B200: 64 sequences with 0 to 4 drafts, 151936 ids, bf16: 21 us for 58 MB of logits and 20 us for the
 // draws (39 MB of noise), both bound by their instructions (14 a logit in the first); 24 sequences with a draft model's
 // probabilities in fp32 13 + 17 us; one sequence 15 us, a chain of dependent loads.
+#include <cfloat>
+
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -165,6 +168,11 @@ struct VerifyArgs {
   int* status;
 };
 
+__device__ __forceinline__ float heat_of(const VerifyArgs& a, int b) {
+  const float t = a.temperature[b];
+  return t > 0.f ? fminf(fmaxf(t, FLT_MIN), FLT_MAX) : t;
+}
+
 // Rows of sequence b: the first one and the number of drafts, -1 where they do not lie in the logits.
 __device__ __forceinline__ int2 rows_of(const VerifyArgs& a, int b) {
   const int r0 = a.cu[b], r1 = a.cu[b + 1];  // compared with the ends before they are subtracted: nothing overflows
@@ -179,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const __grid_c
   pdl_trigger();
   const int part = blockIdx.x, j = blockIdx.y, b = blockIdx.z;
   if (part == 0 && j == 0 && threadIdx.x == 0) a.done[b] = 0;
-  const float heat = a.temperature[b];
+  const float heat = heat_of(a, b);
   const int2 r = rows_of(a, b);
   if (j > r.y) return;
   if (threadIdx.x == 0) at = INT_MAX;
@@ -284,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 3) verify_token_kernel(const __grid_
   }
   const T* logits = static_cast<const T*>(a.logits) + (size_t)r.x * a.V;
   const Q* probs = static_cast<const Q*>(a.draft_probs);
-  const float heat = a.temperature[b];
+  const float heat = heat_of(a, b);
   const bool greedy = !(heat > 0.f);
   // p of id v under row j
   auto p_of = [&](float x, int v, int j) {

@@ -285,7 +285,8 @@ def verify_sampled(logits, cu, drafts, uniforms, noise, temperature, draft_probs
 
     logits [rows, V] bf16 or fp32: rows cu[b] .. cu[b + 1] - 1 are sequence b's, one for each of its drafts and one
     more (cu int32 [B + 1]); drafts int64 [B, K]; uniforms fp32 [B, K] in [0, 1); noise fp32 [B, V] ~ Exp(1);
-    temperature fp32 [B] (<= 0: greedy); draft_probs [B, K, V] fp32 or bf16: the distributions that the drafts were
+    temperature fp32 [B] (<= 0: greedy; others count as 2^-126 at least and as the largest finite number at most);
+    draft_probs [B, K, V] fp32 or bf16: the distributions that the drafts were
     drawn from (omitted: the drafts were certain, as n-gram drafts are).
 
     With p = softmax(logits / temperature), draft d is accepted where u q(d) < p(d).  At the first refusal the next

@@ -282,7 +282,9 @@ def verify_sampled(logits, cu, drafts, uniforms, noise, temperature, draft_probs
         e = torch.where(x == top, 1.0, torch.exp((x - top) / t))
         return e / e.sum()
 
-    offs, heat, us, ds = cu.tolist(), temperature.tolist(), uniforms.cpu(), drafts.tolist()
+    lim = torch.finfo(torch.float32)
+    heat = torch.where(temperature > 0, temperature.clamp(lim.tiny, lim.max), temperature).tolist()
+    offs, us, ds = cu.tolist(), uniforms.cpu(), drafts.tolist()
     for b in range(B):
         n, a = offs[b + 1] - offs[b] - 1, 0
         while True:

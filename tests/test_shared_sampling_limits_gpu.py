@@ -160,3 +160,27 @@ def test_attn_shared_buffers_off_their_alignment_are_refused(N):
             C.attn_shared(b.q, b.k, b.v, b.tables, 1, plan, work, out, scale)
     C.attn_shared(b.q, b.k, b.v, b.tables, 1, p.buf, ws[8:], out, scale)
     b.check(out)
+
+
+HEATS = [1e-45, 1e-40, 4e-39, 2 ** -126, 1e-30, 1e30, torch.finfo(torch.float32).max, math.inf]
+
+
+@pytest.mark.parametrize("q_dtype", [None, torch.float32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_verify_temperatures_at_the_ends(N, dtype, q_dtype):
+    # all of the probability on the largest logit at one end, the same for every id at the other
+    x = Drafts([2] * len(HEATS), 1000, HEATS, seed=21, dtype=dtype, q_dtype=q_dtype)
+    x.check(x.run(N))
+
+
+def test_verify_infinite_temperature_and_masks(N):
+    # masked ids stay out however hot the rest is
+    x = Drafts([1, 1, 0], 1000, [math.inf, torch.finfo(torch.float32).max, math.inf], seed=22)
+    x.logits[:, 100:] = -math.inf
+    x.logits[:, 100] = torch.finfo(torch.float32).min
+    x.drafts[:] = 500
+    acc, tok, probs = x.run(N)
+    want = R.verify_sampled(x.logits, x.cu, x.drafts, x.uniforms, x.noise, x.heat)
+    assert torch.equal(acc, want[0]) and torch.equal(tok, want[1])
+    assert acc.tolist() == [0, 0, 0] and 0 <= int(tok.min()) and int(tok.max()) <= 100
+    assert (probs[:, 0] > 0).all() and torch.allclose(probs, want[2], rtol=2 ** -18, atol=0)
