@@ -184,3 +184,37 @@ def test_verify_infinite_temperature_and_masks(N):
     assert torch.equal(acc, want[0]) and torch.equal(tok, want[1])
     assert acc.tolist() == [0, 0, 0] and 0 <= int(tok.min()) and int(tok.max()) <= 100
     assert (probs[:, 0] > 0).all() and torch.allclose(probs, want[2], rtol=2 ** -18, atol=0)
+
+
+def fine_errors(b, out):
+    """Largest errors over sum(p |v|) beyond the output's last rounding: of ``out``, and of what weights rounded to one
+    bf16 would give."""
+    T, Hq, D = b.q.shape
+    rep, worst = Hq // b.k.shape[1], [0.0, 0.0]
+    for s, c in enumerate(b.ctx):
+        t0, t1 = b.cu[s], b.cu[s + 1]
+        k = R.gather_kv(b.k, b.tables[s], c).double().repeat_interleave(rep, 1)
+        v = R.gather_v(b.v, b.tables[s], c).double().repeat_interleave(rep, 1)
+        x = torch.einsum("qhd,nhd->hqn", b.q[t0:t1].double(), k) / math.sqrt(D)
+        seen = torch.arange(c, device=x.device)[None, :] <= c - (t1 - t0) + torch.arange(t1 - t0, device=x.device)[:, None]
+        x = x.masked_fill(~seen[None], -math.inf)
+        p = torch.softmax(x, -1)
+        o, size = torch.einsum("hqn,nhd->qhd", p, v), torch.einsum("hqn,nhd->qhd", p, v.abs())
+        e = torch.exp(x - x.amax(-1, keepdim=True))
+        one = torch.einsum("hqn,nhd->qhd", e.bfloat16().double() / e.sum(-1, keepdim=True), v).bfloat16()
+        for i, got in enumerate((out[t0:t1], one)):
+            worst[i] = max(worst[i], float((((got.double() - o).abs() - 2 ** -8 * o.abs()) / size).max()))
+    return worst
+
+
+# Values are 1 or -1, so that sums of them cancel and the output's own rounding, 2^-8 of it, hides little.  A key's weight as
+# one bf16 is off by up to 2^-8 of itself; as two bf16 terms by 2^-16, and the exponentials and sums in 32 bits add a few
+# 2^-22 for scores of a few units.
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("groups", [[(0, [(40, 1), (33, 4)])], [(0, [(150, 90), (130, 130)])], [(256, [(1, 1)] * 4)],
+                                    [(112, [(1, 1)] * 70)]], ids=["few rows", "many rows", "prefix", "prefix of part tiles"])
+def test_weights_keep_sixteen_bits(N, D, groups):
+    b = Batch(groups, 8, 2, D, seed=31, q_scale=1.0)
+    b.v.copy_(torch.where(b.v > 0, 1.0, torch.where(b.v <= 0, -1.0, b.v.float())))  # NaN stays where no token is
+    mine, one_term = fine_errors(b, N.attn_shared(b.q, b.k, b.v, b.tables, b.plan(N)))
+    assert mine <= 2 ** -15 < 2 ** -14 < one_term
