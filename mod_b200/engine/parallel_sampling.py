@@ -20,6 +20,7 @@ from typing import List, Optional, Sequence as Seq
 import numpy as np
 import torch
 
+from ..ops import check_status
 from .batch import ForwardBatch
 from .sampler import filter_logits
 from .sequence import SamplingParams, Sequence, SeqStatus
@@ -72,6 +73,8 @@ class ParallelSampler:
         acc, tok, _ = ops.verify_sampled(logits.contiguous(), cu, ids, uniforms, noise,
                                          torch.tensor(heat, dtype=torch.float32).to(dev))
         acc, tok = torch.stack([acc.long(), tok]).tolist()
+        if self.native:   # the step is over on the device: what a kernel gave up on is not emitted
+            check_status(logits.device)
         if min(tok, default=0) < 0:
             raise RuntimeError("a row of logits has no finite entry")
         return acc, tok

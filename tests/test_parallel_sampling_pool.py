@@ -1,0 +1,51 @@
+"""Several continuations of one prompt in an engine that has other work, little room or trouble."""
+import pytest
+import torch
+
+from mod_b200.engine.parallel_sampling import ParallelSampler
+from mod_b200.engine.sequence import SamplingParams
+from tests.test_parallel_sampling import _engine, _prompts
+
+
+def whole(eng):
+    return (eng.blocks.num_free == eng.blocks.num_blocks and not eng.blocks.owners
+            and len(eng.blocks.free_slots) == eng.blocks.max_seqs)
+
+
+# ------------------------------------------------------------------ a kernel that gives up
+def test_status_is_read_every_step(monkeypatch):
+    from mod_b200.engine import parallel_sampling as M
+
+    seen = []
+    monkeypatch.setattr(M, "check_status", lambda dev: seen.append(dev))
+    eng = _engine()
+    s = ParallelSampler(eng)
+    s.native = True               # as on the GPU, with the plain operators in the kernels' place
+    from mod_b200.ops import reference
+
+    eng.backend.N = reference
+    s.generate(_prompts()[:2], 2, SamplingParams(max_new_tokens=6))
+    assert len(seen) == s.stats.steps + 1
+
+    def fail(dev):
+        raise RuntimeError("mbarrier wait timed out")
+
+    monkeypatch.setattr(M, "check_status", fail)
+    with pytest.raises(RuntimeError, match="timed out"):
+        s.generate(_prompts()[:2], 2, SamplingParams(max_new_tokens=6))
+    assert whole(eng)
+
+
+@pytest.mark.gpu
+def test_native_status_ends_the_call():
+    from mod_b200.ops import native as N
+
+    eng = _engine("native", "cuda:0", fp32=False)
+    p = SamplingParams(max_new_tokens=6)
+    want = eng.generate_parallel(_prompts()[:2], 2, p)
+    far = torch.tensor([10 ** 6], dtype=torch.int32, device="cuda")
+    N.kv_copy_pages(eng.kv.k, eng.kv.v, far, far)       # reported, nothing copied
+    with pytest.raises(RuntimeError, match="out of bounds"):
+        eng.generate_parallel(_prompts()[:2], 2, p)
+    assert whole(eng)
+    assert eng.generate_parallel(_prompts()[:2], 2, p) == want
