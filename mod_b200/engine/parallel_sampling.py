@@ -190,7 +190,9 @@ class ParallelSampler:
                 left = sum(len(g) for g in running)
                 if not left:
                     break
-                if 2 * left <= most:  # many have finished: their blocks lie between those that stay
+                # many have finished: their blocks lie between those that stay (with prefix caching too, but there a
+                # compaction would give up the cached blocks of everyone's prompts)
+                if 2 * left <= most and not eng.prefix_caching:
                     eng.compact_kv([c for g in running for c in g])
                     most = left
                 self._step(running, shared)

@@ -49,3 +49,20 @@ def test_native_status_ends_the_call():
         eng.generate_parallel(_prompts()[:2], 2, p)
     assert whole(eng)
     assert eng.generate_parallel(_prompts()[:2], 2, p) == want
+
+
+# ------------------------------------------------------------------ what the engine keeps
+def test_prefix_cache_outlives_uneven_ends():
+    ref = _engine().generate(_prompts(), SamplingParams(max_new_tokens=24))
+    eos = ref[0][2]
+    eng = _engine(prefix_caching=True)
+    old = [[700 + i for i in range(40)], [800 + i for i in range(33)]]
+    want = eng.generate(old, SamplingParams(max_new_tokens=4))
+    held = dict(eng.blocks.cache)
+    assert len(held) >= 4
+    got = eng.generate_parallel(_prompts(), 3, SamplingParams(max_new_tokens=24, eos_token_id=eos))
+    assert [g[0] for g in got] == [r[:r.index(eos) + 1] if eos in r else r for r in ref]
+    assert all(eng.blocks.cache.get(h) == b for h, b in held.items())
+    hits = eng.blocks.hits
+    assert eng.generate(old, SamplingParams(max_new_tokens=4)) == want
+    assert eng.blocks.hits - hits == 2 + 2 and whole(eng)
