@@ -61,7 +61,7 @@ class KVCache:
         new id of every block (-1: in no table) and the number of blocks in use."""
         width = max([1] + [len(t) for t in tables])
         rows = torch.tensor([t + [0] * (width - len(t)) for t in tables], dtype=torch.int32).view(len(tables), width)
-        lens = torch.tensor([len(t) * self.block_size for t in tables], dtype=torch.int32)
+        lens = torch.tensor([len(t) * 16 for t in tables], dtype=torch.int32)  # kv_compact's tokens a page, for whole tables
         dev = self.k[0].device
         _, remap, live = self._ops().kv_compact(self.k, self.v, rows.to(dev), lens.to(dev))
         return remap.tolist(), int(live)

@@ -66,3 +66,18 @@ def test_prefix_cache_outlives_uneven_ends():
     hits = eng.blocks.hits
     assert eng.generate(old, SamplingParams(max_new_tokens=4)) == want
     assert eng.blocks.hits - hits == 2 + 2 and whole(eng)
+
+
+def test_compact_counts_sixteen_tokens_a_block_whatever_its_size():
+    from mod_b200.config import get_preset
+    from mod_b200.engine.kv_cache import KVCache
+
+    for bs in (4, 16, 32):
+        kv = KVCache(get_preset("tiny-dense"), 12, "cpu", dtype=torch.float32, block_size=bs)
+        for c in (*kv.k, *kv.v):
+            c.copy_(torch.arange(12.0).view(12, 1, 1, 1).expand_as(c))
+        tables = [[11, 2, 7, 9], [11, 5, 1]]
+        remap, live = kv.compact(tables)
+        assert live == 6 and {remap[b] for t in tables for b in t} == set(range(6))
+        for c in (*kv.k, *kv.v):
+            assert all((c[remap[b]] == b).all() for t in tables for b in t)
