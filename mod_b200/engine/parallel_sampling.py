@@ -205,12 +205,12 @@ class ParallelSampler:
     def generate(self, prompts: List[Seq[int]], n: int, params: Optional[SamplingParams] = None) -> List[List[List[int]]]:
         """``n`` continuations of each prompt.  At most the engine's batch of sequences runs at a time."""
         params = params or SamplingParams()
-        room = self.eng.blocks.max_seqs // (n + 1)   # a slot for each prompt while it is forked
-        if n < 1 or room < 1:
+        if n < 1 or n >= self.eng.blocks.max_seqs:   # a slot for the prompt while it is forked
             raise ValueError(f"n = {n}: between 1 and {self.eng.blocks.max_seqs - 1} (the engine's batch less the prompt's)")
         if any(len(p) < 1 or len(p) + params.max_new_tokens > self.eng.runner.max_blocks * self.eng.blocks.block_size
                for p in prompts):
             raise ValueError("a prompt is empty or does not fit the model length with its new tokens")
+        room = self.eng.blocks.max_seqs // (n + 1)
         self._seed(params)
         out: List[List[List[int]]] = []
         for i in range(0, len(prompts), room):

@@ -81,3 +81,10 @@ def test_compact_counts_sixteen_tokens_a_block_whatever_its_size():
         assert live == 6 and {remap[b] for t in tables for b in t} == set(range(6))
         for c in (*kv.k, *kv.v):
             assert all((c[remap[b]] == b).all() for t in tables for b in t)
+
+
+# ------------------------------------------------------------------ arguments
+@pytest.mark.parametrize("n", [0, -1, -2, -17, 16, 100])
+def test_counts_out_of_range_are_refused(n):
+    with pytest.raises(ValueError, match="n ="):
+        _engine().generate_parallel([[1, 2, 3]], n, SamplingParams(max_new_tokens=4))
