@@ -116,6 +116,9 @@ class ParallelSampler:
     def _step(self, running: List[List[Sequence]], shared: List[int]) -> None:
         eng = self.eng
         seqs = [s for g in running for s in g]
+        for s in seqs:  # everyone's last token first, drafts into what is left
+            if not eng.blocks.allocate(s, s.length):
+                raise RuntimeError("KV cache exhausted during parallel sampling")
         drafts = []
         for s in seqs:
             room = min(self.k, s.params.max_new_tokens - len(s.output) - 1,
@@ -123,8 +126,6 @@ class ParallelSampler:
             d = ngram_propose(s.all_tokens, room, self.nmax, self.nmin) if room > 0 else []
             if d and not eng.blocks.allocate(s, s.length + len(d)):
                 d = []
-            if not eng.blocks.allocate(s, s.length):
-                raise RuntimeError("KV cache exhausted during parallel sampling")
             drafts.append(d)
         logits = self._forward(seqs, drafts, [len(g) for g in running], shared)
         acc, tok = self._verify(logits, [len(d) for d in drafts], drafts, seqs)

@@ -88,3 +88,26 @@ def test_compact_counts_sixteen_tokens_a_block_whatever_its_size():
 def test_counts_out_of_range_are_refused(n):
     with pytest.raises(ValueError, match="n ="):
         _engine().generate_parallel([[1, 2, 3]], n, SamplingParams(max_new_tokens=4))
+
+
+# ------------------------------------------------------------------ little room
+def test_drafts_take_what_the_next_tokens_leave(monkeypatch):
+    from mod_b200.engine import parallel_sampling as M
+    from mod_b200.engine.sequence import Sequence, SeqStatus
+
+    eng = _engine(num_blocks=3)
+    s = ParallelSampler(eng)
+    s._seed(SamplingParams())
+    params = SamplingParams(max_new_tokens=20)
+    p = Sequence(prompt=list(range(1, 15)), params=params)
+    assert eng.blocks.allocate(p, p.length)
+    eng.runner.prefill([p], [p.length])
+    a, b = Sequence(prompt=p.prompt, params=params), Sequence(prompt=p.prompt, params=params)
+    eng.kv.copy_pages(eng.blocks.fork(p, a) + eng.blocks.fork(p, b))
+    eng.blocks.release(p)
+    a.output, b.output = [7], [7, 8, 9]           # b's last token needs the one free block, a's drafts would like it
+    a.status = b.status = SeqStatus.RUNNING
+    monkeypatch.setattr(M, "ngram_propose", lambda tokens, room, *n: [5] * room)
+    s._step([[a, b]], [0])
+    assert len(a.output) == 2 and len(b.blocks) == 2 and len(a.blocks) == 1
+    assert s.stats.drafted > 0                     # b drafted into the rest of its block
