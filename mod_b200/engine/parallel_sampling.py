@@ -149,17 +149,46 @@ class ParallelSampler:
         self.stats.per_step.append(n)
 
     # ------------------------------------------------------------------ a wave of prompts
+    def _admit(self, prompts: List[Seq[int]], n: int, params: SamplingParams, parents: List[Sequence]) -> None:
+        """Gives blocks to the first prompts, as many as can be forked into n sequences each now, and appends them to
+        ``parents``.  Where other requests hold what the first one needs, they are run until it is there."""
+        eng, m = self.eng, self.eng.blocks
+        forks = 0   # blocks that the forks will take: a copy of each partly filled last block
+        for p in prompts:
+            s = Sequence(prompt=[int(t) for t in p], params=params)
+            more = n if s.length % m.block_size else 0
+
+            def fits() -> bool:
+                if not m.allocate(s, s.length):
+                    return False
+                if m.num_free >= forks + more and len(m.free_slots) >= n * (len(parents) + 1):
+                    return True
+                m.release(s)
+                return False
+
+            ok = fits()
+            while not ok and not parents and eng.scheduler.running:
+                eng.step()
+                ok = fits()
+            if not ok:
+                if not parents:
+                    raise RuntimeError(f"KV cache exhausted: a prompt of {s.length} tokens and its {n} continuations do not fit")
+                return
+            parents.append(s)
+            forks += more
+
     def _wave(self, prompts: List[Seq[int]], n: int, params: SamplingParams) -> List[List[List[int]]]:
+        """The continuations of the first prompts, of as many as there is room for."""
         eng, bs = self.eng, self.eng.blocks.block_size
-        parents = [Sequence(prompt=[int(t) for t in p], params=params) for p in prompts]
-        children = [[Sequence(prompt=list(p.prompt), params=params) for _ in range(n)] for p in parents]
+        parents: List[Sequence] = []
+        children: List[List[Sequence]] = []
         try:
+            self._admit(prompts, n, params, parents)
+            children += [[Sequence(prompt=list(p.prompt), params=params) for _ in range(n)] for p in parents]
             rows, at = [], 0
             while at < len(parents):  # the prompts, as many at a time as a prefill step takes
                 end, tokens = at, 0
                 while end < len(parents) and (end == at or tokens + parents[end].length <= eng.scheduler.max_prefill_tokens):
-                    if not eng.blocks.allocate(parents[end], parents[end].length):
-                        raise RuntimeError("KV cache exhausted during parallel sampling")
                     tokens += parents[end].length - parents[end].num_cached
                     end += 1
                 part = parents[at:end]
@@ -204,16 +233,16 @@ class ParallelSampler:
                     eng.blocks.release(s)
 
     def generate(self, prompts: List[Seq[int]], n: int, params: Optional[SamplingParams] = None) -> List[List[List[int]]]:
-        """``n`` continuations of each prompt.  At most the engine's batch of sequences runs at a time."""
+        """``n`` continuations of each prompt.  The prompts come in waves, each of as many as there are free blocks and
+        places in the engine's batch to begin with; the continuations of a prompt begin together."""
         params = params or SamplingParams()
         if n < 1 or n >= self.eng.blocks.max_seqs:   # a slot for the prompt while it is forked
             raise ValueError(f"n = {n}: between 1 and {self.eng.blocks.max_seqs - 1} (the engine's batch less the prompt's)")
         if any(len(p) < 1 or len(p) + params.max_new_tokens > self.eng.runner.max_blocks * self.eng.blocks.block_size
                for p in prompts):
             raise ValueError("a prompt is empty or does not fit the model length with its new tokens")
-        room = self.eng.blocks.max_seqs // (n + 1)
         self._seed(params)
         out: List[List[List[int]]] = []
-        for i in range(0, len(prompts), room):
-            out += self._wave(prompts[i:i + room], n, params)
+        while len(out) < len(prompts):
+            out += self._wave(prompts[len(out):], n, params)
         return out

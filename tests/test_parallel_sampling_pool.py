@@ -111,3 +111,41 @@ def test_drafts_take_what_the_next_tokens_leave(monkeypatch):
     s._step([[a, b]], [0])
     assert len(a.output) == 2 and len(b.blocks) == 2 and len(a.blocks) == 1
     assert s.stats.drafted > 0                     # b drafted into the rest of its block
+
+
+@pytest.mark.parametrize("caching", [False, True])
+@pytest.mark.parametrize("blocks", [5, 6, 8, 11, 20])
+def test_prompts_wait_for_blocks(blocks, caching):
+    # 40 tokens: two full blocks and one that is copied for each of two continuations; 8 more tokens fit the copies
+    P = [[(31 * i + 7 * j) % 500 + 1 for j in range(40)] for i in range(5)]
+    params = SamplingParams(max_new_tokens=8)
+    ref = _engine(num_blocks=blocks).generate(P, params)
+    eng = _engine(num_blocks=blocks, prefix_caching=caching)
+    assert eng.generate_parallel(P, 2, params) == [[r] * 2 for r in ref]
+    assert whole(eng)
+
+
+def test_prompts_wait_for_places():
+    P = [[(31 * i + 7 * j) % 500 + 1 for j in range(20)] for i in range(7)]
+    params = SamplingParams(max_new_tokens=6)
+    ref = _engine().generate(P, params)
+    for n in (1, 5, 7, 8, 15):    # a batch of 16
+        eng = _engine()
+        assert eng.generate_parallel(P, n, params) == [[r] * n for r in ref]
+        assert whole(eng)
+
+
+@pytest.mark.parametrize("blocks", [7, 9])
+def test_other_requests_hold_the_blocks(blocks):
+    # two requests are under way when the call comes; it needs five blocks, and they are run until these are free
+    P = [[(31 * i + 7 * j) % 500 + 1 for j in range(40)] for i in range(3)]
+    params = SamplingParams(max_new_tokens=8)
+    ref = _engine().generate(P, params)
+    eng = _engine(num_blocks=blocks)
+    ids = [eng.add_request(p, params) for p in P[:2]]
+    eng.step()
+    assert eng.scheduler.running
+    assert eng.generate_parallel(P[2:], 2, params) == [[ref[2]] * 2]
+    while eng.has_unfinished():
+        eng.step()
+    assert [eng.seqs[i].output for i in ids] == ref[:2] and whole(eng)
