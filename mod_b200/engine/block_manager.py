@@ -64,11 +64,12 @@ class BlockManager:
     def _take(self) -> int:
         return self.free.pop()
 
-    def fork(self, parent: Sequence, child: Sequence) -> Optional[List[Tuple[int, int]]]:
-        """``child`` (without blocks) continues ``parent``'s cached tokens: it shares the full blocks, and the partly
-        filled last one is to be copied.  Returns the (source, target) pairs of that copy, or None where no block or
-        slot is free.  Full blocks are never written again, so sharing needs no further care."""
-        full, part = divmod(parent.num_cached, self.block_size)
+    def fork(self, parent: Sequence, child: Sequence, tokens: Optional[int] = None) -> Optional[List[Tuple[int, int]]]:
+        """``child`` (without blocks) continues ``parent``'s cached tokens, or its first ``tokens``: it shares the full
+        blocks, and the partly filled last one is to be copied.  Returns the (source, target) pairs of that copy, or None
+        where no block or slot is free.  Full blocks are never written again, so sharing needs no further care."""
+        tokens = parent.num_cached if tokens is None else tokens
+        full, part = divmod(tokens, self.block_size)
         if child.blocks or (part and self.num_free < 1) or (child.state_slot < 0 and not self.free_slots):
             return None
         child.blocks = list(parent.blocks[:full])
@@ -80,7 +81,7 @@ class BlockManager:
             pairs.append((parent.blocks[full], child.blocks[full]))
         if child.state_slot < 0:
             child.state_slot = self.free_slots.pop()
-        child.num_cached = parent.num_cached
+        child.num_cached = tokens
         return pairs
 
     def _share(self, block: int) -> None:
@@ -189,10 +190,10 @@ class PrefixCachingBlockManager(BlockManager):
         seq.num_cached = 0
         seq.registered = 0
 
-    def fork(self, parent: Sequence, child: Sequence):
-        pairs = super().fork(parent, child)
+    def fork(self, parent: Sequence, child: Sequence, tokens: Optional[int] = None):
+        pairs = super().fork(parent, child, tokens)
         if pairs is not None:
-            child.registered = getattr(parent, "registered", 0)
+            child.registered = min(getattr(parent, "registered", 0), child.num_cached // self.block_size)
         return pairs
 
     def _share(self, block: int) -> None:

@@ -9,6 +9,9 @@
    emitted tokens follow the same distribution as sampling one token after another, greedy requests give the greedy
    tokens.  KV entries of refused drafts are overwritten later.
 
+Where the blocks run out, the newest continuations give theirs back and come back later: forked again from the prompt, with
+what they had emitted computed in one step before they go on.
+
 On other backends than the native one the same steps run on the plain restatements of the operators.  Attention-only
 models in a single process, as for n-gram speculation: recurrent state can neither be shared nor rolled back.
 """
@@ -85,16 +88,18 @@ class ParallelSampler:
         ``shared``: tokens whose blocks they have in common."""
         r = self.eng.runner
         bs, dev = r.blocks.block_size, r.device
-        ids, pos, slots, ctx, qlens = [], [], [], [], []
+        ids, pos, slots, ctx, qlens, rows = [], [], [], [], [], []
         bt = np.zeros((len(seqs), r.max_blocks), dtype=np.int32)
         for i, (s, d) in enumerate(zip(seqs, drafts)):
-            start = s.length - 1                     # the last emitted token is not cached yet
-            p = np.arange(start, start + 1 + len(d))
-            ids += [s.last_token] + d
+            start = s.num_cached      # the last emitted token is not cached yet, nor others after a time without blocks
+            toks = s.output[start - len(s.prompt):] + d
+            p = np.arange(start, start + len(toks))
+            ids += toks
             pos.append(p)
             slots.append(np.asarray(s.blocks)[p // bs] * bs + p % bs)
-            ctx.append(start + 1 + len(d))
-            qlens.append(1 + len(d))
+            ctx.append(start + len(toks))
+            qlens.append(len(toks))
+            rows += range(len(ids) - 1 - len(d), len(ids))
             bt[i, :len(s.blocks)] = s.blocks
 
         def up(x, dtype=torch.int32):
@@ -103,7 +108,7 @@ class ParallelSampler:
         T = len(ids)
         fb = ForwardBatch(input_ids=up(ids, torch.long), positions=up(np.concatenate(pos)),
                           slot_mapping=up(np.concatenate(slots)), block_tables=torch.from_numpy(bt).to(dev),
-                          ctx_lens=up(ctx), logits_idx=torch.arange(T, device=dev),
+                          ctx_lens=up(ctx), logits_idx=up(rows, torch.long),
                           state_slots=up([s.state_slot for s in seqs], torch.long), is_decode=False, query_lens=qlens,
                           ctx_lens_host=ctx)
         if self.shared:  # one schedule for all layers of the step
@@ -113,12 +118,72 @@ class ParallelSampler:
                 self.eng.cfg.head_dim, cu_q=up(np.cumsum([0] + qlens)))
         return r.model.logits(r.model.forward(fb, r.kv, r.states))
 
+    def _make_room(self, seqs: List[Sequence]) -> None:
+        """Blocks for everyone's last token; where they do not suffice, the newest sequences give theirs back."""
+        eng = self.eng
+        for s in seqs:
+            while s.status == SeqStatus.RUNNING and not eng.blocks.allocate(s, s.length):
+                running = [x for x in seqs if x.status == SeqStatus.RUNNING]
+                if len(running) > 1:
+                    eng.blocks.release(running[-1])
+                    running[-1].status = SeqStatus.WAITING
+                    eng.scheduler.num_preempted += 1
+                elif eng.scheduler.running:    # other requests hold the rest
+                    eng.step()
+                else:
+                    raise RuntimeError("KV cache exhausted during parallel sampling")
+
+    def _most_blocks(self, s: Sequence) -> int:
+        return self.eng.blocks.blocks_needed(max(s.length, len(s.prompt) + s.params.max_new_tokens - 1))
+
+    def _resume(self, children: List[List[Sequence]]) -> None:
+        """Forks sequences without blocks again, in order: while everyone who runs would still find all the blocks that
+        it can come to need, so that none is computed anew more than once, and always one where nobody runs."""
+        eng, m = self.eng, self.eng.blocks
+        running = [c for cs in children for c in cs if c.status == SeqStatus.RUNNING]
+        tokens = 0   # that are computed again in this step
+        for cs in children:
+            for c in cs:
+                if c.status != SeqStatus.WAITING:
+                    continue
+                other = next((x for x in cs if x.status == SeqStatus.RUNNING), None)
+                if running:
+                    need = sum(self._most_blocks(x) - len(x.blocks) for x in running) + self._most_blocks(c)
+                    need += 1 if other is None else -(len(c.prompt) // m.block_size)
+                    if (need > m.num_free or len(m.free_slots) < 1 + (other is None)
+                            or tokens + len(c.output) > eng.scheduler.max_prefill_tokens):
+                        return
+                if other is not None:
+                    pairs = m.fork(other, c, len(c.prompt))
+                    eng.kv.copy_pages(pairs)
+                else:
+                    self._fork_anew(c)
+                c.status = SeqStatus.RUNNING
+                running.append(c)
+                tokens += len(c.output)
+
+    def _fork_anew(self, c: Sequence) -> None:
+        """The prompt of ``c`` once more, for it alone."""
+        eng, parents = self.eng, []
+        try:
+            self._admit([c.prompt], 1, c.params, parents)
+            p = parents[0]
+            eng.runner.prefill([p], [p.length - p.num_cached], return_logits=True)
+            if eng.prefix_caching:
+                eng.blocks.register(p)
+            eng.kv.copy_pages(eng.blocks.fork(p, c))
+        finally:
+            for p in parents:
+                eng.blocks.release(p)
+
     def _step(self, running: List[List[Sequence]], shared: List[int]) -> None:
         eng = self.eng
+        # everyone's last token first, drafts into what is left
+        self._make_room([s for g in running for s in g])
+        running = [[s for s in g if s.status == SeqStatus.RUNNING] for g in running]
+        shared = [n for n, g in zip(shared, running) if g]
+        running = [g for g in running if g]
         seqs = [s for g in running for s in g]
-        for s in seqs:  # everyone's last token first, drafts into what is left
-            if not eng.blocks.allocate(s, s.length):
-                raise RuntimeError("KV cache exhausted during parallel sampling")
         drafts = []
         for s in seqs:
             room = min(self.k, s.params.max_new_tokens - len(s.output) - 1,
@@ -214,12 +279,13 @@ class ParallelSampler:
                 self._emit(c, [t])
             most = len(every)
             while True:
+                self._resume(children)
                 running = [[c for c in cs if c.status == SeqStatus.RUNNING] for cs in children]
                 shared = [len(p.prompt) // bs * bs for p, g in zip(parents, running) if g]
                 running = [g for g in running if g]
-                left = sum(len(g) for g in running)
-                if not left:
+                if not running:
                     break
+                left = sum(c.status != SeqStatus.FINISHED for c in every)
                 # many have finished: their blocks lie between those that stay (with prefix caching too, but there a
                 # compaction would give up the cached blocks of everyone's prompts)
                 if 2 * left <= most and not eng.prefix_caching:

@@ -149,3 +149,52 @@ def test_other_requests_hold_the_blocks(blocks):
     while eng.has_unfinished():
         eng.step()
     assert [eng.seqs[i].output for i in ids] == ref[:2] and whole(eng)
+
+
+@pytest.mark.parametrize("caching", [False, True])
+@pytest.mark.parametrize("drafts", [0, 3])
+@pytest.mark.parametrize("blocks", range(8, 22))
+def test_sequences_that_outgrow_the_pool_come_back(blocks, drafts, caching):
+    # what generate() does with the same sequences one beside another in the same pool
+    P, params = _prompts()[:3], SamplingParams(max_new_tokens=20)
+    ref = _engine(num_blocks=blocks).generate([p for p in P for _ in range(3)], params)
+    eng = _engine(num_blocks=blocks, prefix_caching=caching)
+    s = ParallelSampler(eng, drafts=drafts)
+    assert [x for g in s.generate(P, 3, params) for x in g] == ref
+    assert whole(eng)
+
+
+def test_each_sequence_is_computed_again_once_at_most():
+    P, params = _prompts()[:3], SamplingParams(max_new_tokens=60)
+    ref = _engine().generate(P, params)
+    eng = _engine(num_blocks=14)
+    s = ParallelSampler(eng)
+    back = []
+    fork = eng.blocks.fork
+    eng.blocks.fork = lambda p, c, *n: (back.append(c.req_id) if c.output else None) or fork(p, c, *n)
+    assert s.generate(P, 4, params) == [[r] * 4 for r in ref]
+    assert back and len(set(back)) == len(back) and eng.scheduler.num_preempted >= len(back)
+
+
+def test_one_sequence_that_does_not_fit_is_refused():
+    # 36 + 63 cached tokens take 7 blocks
+    P, params = [_prompts()[0]], SamplingParams(max_new_tokens=64)
+    for blocks in (5, 6):
+        eng = _engine(num_blocks=blocks)
+        with pytest.raises(RuntimeError, match="exhausted"):
+            eng.generate_parallel(P, 2, params)
+        assert whole(eng)
+    eng = _engine(num_blocks=7)
+    assert eng.generate_parallel(P, 2, params) == [_engine().generate(P, params) * 2] and whole(eng)
+
+
+def test_growth_beside_other_requests():
+    P, params = _prompts()[:3], SamplingParams(max_new_tokens=40)
+    ref = _engine().generate(P, params)
+    eng = _engine(num_blocks=11)
+    rid = eng.add_request(P[2], params)
+    eng.step()
+    assert eng.generate_parallel(P[:2], 2, params) == [[r] * 2 for r in ref[:2]]
+    while eng.has_unfinished():
+        eng.step()
+    assert eng.seqs[rid].output == ref[2] and whole(eng)
