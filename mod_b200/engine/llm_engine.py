@@ -481,7 +481,8 @@ class LLMEngine:
 
     def generate_parallel(self, prompts: List[Seq[int]], n: int, params: Optional[SamplingParams] = None,
                           drafts: int = 4) -> List[List[List[int]]]:
-        """``n`` continuations of each prompt, computed once and forked; see ``engine.parallel_sampling``."""
+        """``n`` continuations of each prompt, computed once and forked; see ``engine.parallel_sampling``.  With a seed,
+        a prompt's continuations do not depend on the call's other prompts."""
         from .parallel_sampling import ParallelSampler
 
         return ParallelSampler(self, drafts=drafts).generate(prompts, n, params)

@@ -17,8 +17,9 @@ models in a single process, as for n-gram speculation: recurrent state can neith
 """
 from __future__ import annotations
 
+import random
 import time
-from typing import List, Optional, Sequence as Seq
+from typing import Dict, List, Optional, Sequence as Seq, Tuple
 
 import numpy as np
 import torch
@@ -42,6 +43,7 @@ class ParallelSampler:
         self.shared = self.native and engine.cfg.head_dim in (64, 128, 256)
         self.stats = SpecStats()
         self.gen: Optional[torch.Generator] = None
+        self.gens: Dict[int, Tuple[random.Random, torch.Generator]] = {}    # of seeded sequences, by request id
 
     # ------------------------------------------------------------------ random numbers
     def _seed(self, params: SamplingParams) -> None:
@@ -50,6 +52,21 @@ class ParallelSampler:
             self.gen.manual_seed(params.seed)
         else:
             self.gen.seed()
+
+    def _draw(self, seqs: List[Sequence], K: int, V: int):
+        """Uniforms [B, K] and Exp(1) noise [B, V].  Seeded sequences have generators of their own, which depend on the
+        seed and on a sequence's place among its prompt's continuations, and draw as much in every step: what is emitted
+        does not change with the other sequences.  It costs a launch a sequence (0.4 ms a step for 63 of 151936 ids)."""
+        dev, B = self.eng.device, len(seqs)
+        noise = torch.empty(B, V, device=dev)
+        if not self.gens:
+            return torch.rand(B, K, device=dev, generator=self.gen), noise.exponential_(generator=self.gen)
+        rows = []
+        for z, s in zip(noise, seqs):
+            host, g = self.gens[s.req_id]
+            rows.append([host.getrandbits(24) / 2 ** 24 for _ in range(max(1, self.k))][:K])
+            z.exponential_(generator=g)
+        return torch.tensor(rows).to(dev), noise
 
     # ------------------------------------------------------------------ verification
     def _verify(self, logits: torch.Tensor, counts: List[int], drafts: List[List[int]], seqs: List[Sequence]):
@@ -67,8 +84,7 @@ class ParallelSampler:
             heat = [1.0 if t > 0 else 0.0 for t in heat]
         cu = torch.tensor(np.cumsum([0] + [c + 1 for c in counts]), dtype=torch.int32).to(dev)
         ids = torch.tensor([d + [0] * (K - len(d)) for d in drafts], dtype=torch.long).view(B, K).to(dev)
-        uniforms = torch.rand(B, K, device=dev, generator=self.gen)
-        noise = torch.empty(B, logits.shape[1], device=dev).exponential_(generator=self.gen)
+        uniforms, noise = self._draw(seqs, K, logits.shape[1])
         if self.native:
             ops = self.eng.backend.N
         else:
@@ -250,6 +266,12 @@ class ParallelSampler:
         try:
             self._admit(prompts, n, params, parents)
             children += [[Sequence(prompt=list(p.prompt), params=params) for _ in range(n)] for p in parents]
+            if params.seed is not None and params.temperature > 0:
+                for cs in children:
+                    for i, c in enumerate(cs):
+                        host = random.Random(f"{params.seed} {i}")
+                        self.gens[c.req_id] = host, torch.Generator(device=eng.device)
+                        self.gens[c.req_id][1].manual_seed(host.getrandbits(63))
             rows, at = [], 0
             while at < len(parents):  # the prompts, as many at a time as a prefill step takes
                 end, tokens = at, 0
@@ -297,6 +319,7 @@ class ParallelSampler:
             for s in [*parents, *(c for cs in children for c in cs)]:
                 if s.blocks or s.state_slot >= 0:
                     eng.blocks.release(s)
+                self.gens.pop(s.req_id, None)
 
     def generate(self, prompts: List[Seq[int]], n: int, params: Optional[SamplingParams] = None) -> List[List[List[int]]]:
         """``n`` continuations of each prompt.  The prompts come in waves, each of as many as there are free blocks and

@@ -198,3 +198,46 @@ def test_growth_beside_other_requests():
     while eng.has_unfinished():
         eng.step()
     assert eng.seqs[rid].output == ref[2] and whole(eng)
+
+
+# ------------------------------------------------------------------ seeds
+@pytest.mark.parametrize("drafts", [0, 4])
+def test_seeded_continuations_do_not_depend_on_the_other_prompts(drafts):
+    P, params = _prompts(), SamplingParams(max_new_tokens=16, temperature=0.9, seed=11)
+    run = lambda prompts, n=3, **kw: ParallelSampler(_engine(**kw), drafts=drafts).generate(prompts, n, params)  # noqa: E731
+    alone = [run([p])[0] for p in P]
+    assert run(P) == alone and run(P[::-1]) == alone[::-1] and run([P[2], P[0]]) == [alone[2], alone[0]]
+    assert [g[:2] for g in alone] == run(P, 2)            # nor on how many there are
+    assert len({tuple(x) for g in alone for x in g}) == len(P) * 3
+    # a call on the same engine repeats it, one with another seed does not
+    s = ParallelSampler(_engine(), drafts=drafts)
+    assert s.generate(P[:1], 3, params) == s.generate(P[:1], 3, params) == alone[:1] and not s.gens
+    assert s.generate(P[:1], 3, SamplingParams(max_new_tokens=16, temperature=0.9, seed=12)) != alone[:1]
+
+
+@pytest.mark.gpu
+def test_native_seeded_continuations_do_not_depend_on_the_other_prompts():
+    # bf16 rounds with the batch a prompt is computed in, so that a later token may differ by that alone: the first one,
+    # drawn from the prompt's own logits, has to be the same for most, and every one for the same call
+    P, params = _prompts(), SamplingParams(max_new_tokens=8, temperature=0.9, seed=11)
+    run = lambda prompts: _engine("native", "cuda:0", fp32=False).generate_parallel(prompts, 4, params)  # noqa: E731
+    a, b = run(P), run(P[::-1])[::-1]
+    first = [x[0] == y[0] for g, h in zip(a, b) for x, y in zip(g, h)]
+    assert sum(first) >= len(first) - 1 and run(P) == a
+
+
+def test_unseeded_continuations_differ():
+    params = SamplingParams(max_new_tokens=12, temperature=1.0)
+    s = ParallelSampler(_engine())
+    got = [x for _ in range(2) for g in s.generate(_prompts()[:2], 4, params) for x in g]
+    assert len({tuple(x) for x in got}) > 12
+
+
+def test_sampled_sequences_that_come_back_go_on_as_they_were():
+    # sampled tokens do not depend on when a sequence had blocks, without drafts
+    P, params = _prompts()[:3], SamplingParams(max_new_tokens=30, temperature=1.0, top_k=40, seed=9)
+    want = ParallelSampler(_engine(), drafts=0).generate(P, 3, params)
+    small = _engine(num_blocks=9)
+    got = ParallelSampler(small, drafts=0).generate(P, 3, params)
+    assert small.scheduler.num_preempted > 0 and whole(small)
+    assert all(len(x) == 30 for g in got for x in g) and got == want
