@@ -241,3 +241,30 @@ def test_sampled_sequences_that_come_back_go_on_as_they_were():
     got = ParallelSampler(small, drafts=0).generate(P, 3, params)
     assert small.scheduler.num_preempted > 0 and whole(small)
     assert all(len(x) == 30 for g in got for x in g) and got == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("caching", [False, True])
+def test_native_sequences_that_outgrow_the_pool_come_back(caching):
+    # the computed-again step has as many query tokens as a sequence had emitted, over the shared-prefix kernels
+    from mod_b200.engine.sequence import Sequence
+
+    P, params = _prompts(), SamplingParams(max_new_tokens=90)
+    ref = _engine("native", "cuda:0", fp32=False).generate(P, params)
+    eng = _engine("native", "cuda:0", fp32=False, num_blocks=19, prefix_caching=caching)
+    got = eng.generate_parallel(P, 3, params)
+    assert eng.scheduler.num_preempted > 0 and whole(eng)
+    # Where a continuation leaves the greedy one, the two tokens' logits have to tie, within two bf16 roundings (2^-8 each)
+    # in each of the two paths.
+    for prompt, r, g in zip(P, ref, got):
+        for x in g:
+            assert len(x) == 90
+            k = next((i for i in range(90) if x[i] != r[i]), None)
+            if k is None:
+                continue
+            q = Sequence(prompt=prompt + r[:k], params=SamplingParams())
+            assert eng.blocks.allocate(q, q.length)
+            logits = eng.runner.prefill([q], [q.length - q.num_cached], return_logits=True)[0]
+            eng.blocks.release(q)
+            top = float(logits.max())
+            assert min(float(logits[x[k]]), float(logits[r[k]])) >= top - 2 ** -6 * float(logits.abs().max()), (k, x, r)
