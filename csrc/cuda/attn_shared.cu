@@ -166,6 +166,14 @@ __device__ void block_scan(int* a, int n, int* sh) {
   __syncthreads();
 }
 
+// *total += x of every thread; each thread of the block calls it.  One shared-memory addition a warp: 64-bit ones are retried
+// where threads collide, and 128 sequences made the plan 6 us longer that way.
+__device__ __forceinline__ void add_all(unsigned long long* total, unsigned long long x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+  if ((threadIdx.x & 31) == 0 && x) atomicAdd(total, x);
+}
+
 // The last i of [0, n) with a[i] <= x (a ascending), -1 if there is none.
 __device__ __forceinline__ int last_le(const int* a, int n, int x) {
   int lo = -1, hi = n - 1;
@@ -230,13 +238,15 @@ __global__ void __launch_bounds__(kPlanThreads)
     gu[g] = pre[g] > 0 ? (rows + d.wide_rows - 1) / d.wide_rows : 0;
   }
   __syncthreads();
+  unsigned long long mine = 0;
   for (int b = tid; b < d.B; b += kPlanThreads) {
     const int g = group_of(b), p = g >= 0 ? pre[g] : 0, c = ctx_of(b), rows = (cu[b + 1] - cu[b]) * d.Gq;
     const bool any = c > p && rows > 0, lean = rows <= d.lean_rows;
     su[b] = any && !lean ? (rows + kTileRows - 1) / kTileRows : 0;
     le[b] = any && lean ? (rows + 15) / 16 : 0;
-    if (le[b]) atomicAdd(&lean_pages, (unsigned long long)le[b] * ((c - p + 15) / 16));
+    if (le[b]) mine += (unsigned long long)le[b] * ((c - p + 15) / 16);
   }
+  add_all(&lean_pages, mine);
   __syncthreads();
   // pages of a lean piece: as many pieces as the warps that run them, but no less than kLeanPages
   const int64_t page_work = (int64_t)lean_pages * d.Hkv;
@@ -275,6 +285,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     x.direct = p == 0 && chunks == 1;
     reinterpret_cast<Piece*>(v.lean)[i] = x;
   }
+  mine = 0;
   for (int i = tid; i < n; i += kPlanThreads) {
     Unit u;
     if (i < nG) {
@@ -300,8 +311,9 @@ __global__ void __launch_bounds__(kPlanThreads)
     reinterpret_cast<Unit*>(v.units)[i] = u;
     v.cost[i] = u.tiles * (u.rows > kTileRows ? kCostWide : kCostNarrow) + kCostUnit;
     v.rowcum[i] = u.rows;
-    atomicAdd(&total_cost, (unsigned long long)v.cost[i]);
+    mine += v.cost[i];
   }
+  add_all(&total_cost, mine);
   __syncthreads();
   if (total_cost > INT_MAX) {  // the cuts below are searched for in 32-bit sums: a plan of nothing
     if (tid == 0) set_status(status, kErrBounds);
