@@ -35,14 +35,19 @@
 //
 // Sums, maxima and O are in fp32.  P enters the second product as two bf16 terms (16 bits of it): one term alone makes the
 // whole result's error 1.4 times that of its final rounding, two cost 1 to 4% of the time (132 -> 133 us on 32768 shared
-// tokens under 128 sequences, 33 -> 35 us on 8192 under 64), since the softmax and not the tensor cores bounds a tile.
+// tokens under 128 sequences, 33 -> 35 us on 8192 under 64).
 // Token slots past the context may hold anything: their scores are masked by selection and their V columns are zeroed
 // in shared memory.  Every wait is bounded.
 //
-// Measured on one B200 (whole call in a CUDA graph): 32 heads on 4 KV heads, 32768 shared tokens under 128 sequences with
-// up to 1024 own: 126 to 133 us from run to run, 540 TFLOP/s; bound by the softmax of a 64-key tile (about 1450 clocks in each of two warps an
-// SM quarter, of 1900 a step).  2048 shared under 64 with up to 512 own: 30 us, of which about 12 the own tokens, 11 the
-// prefix (a start of 4500 clocks and 9000 clocks to write 256 partial rows an SM around one step) and the rest the join.
+// Measured on one B200 (a layer's three launches in a CUDA graph; the step's plan is another 10 us, 12 with 128 sequences):
+// 32 heads on 4 KV heads, 32768 shared tokens under 128 sequences with up to 1024 own: 129 to 137 us from run to run, 540
+// TFLOP/s.  A 64-key step of 256 rows takes 2250 clocks more (counters at 8192 and 16384 shared tokens), of which the tensor
+// cores are busy 1570 (three products, one of them for the second term of P) and the special-function units 1024; a tile's
+// chain of product, softmax (about 1450 in each of two warps an SM quarter) and product fills the rest.  55 steps an SM are
+// 63 us at 1965 MHz, 71 at the 1747 that such calls one after another settle at under the power limit; the own tokens take 28
+// before them, starts, partial rows and the join what remains.  2048 shared under 64 with up to 512 own: 29 us, of which
+// about 12 the own tokens, 11 the prefix (a start of 4500 clocks and 9000 clocks to write 256 partial rows an SM around one
+// step) and the rest the join.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <torch/extension.h>

@@ -7,7 +7,7 @@
 // Both are bound by HBM: each moved byte is read and written once.  A copy is a grid of as many CTAs as fit, each taking
 // one page of one tensor after another with up to eight 16-byte loads in flight a thread.  The plan of a compaction is one CTA
 // with the live pages as bits in shared memory.  Measured on one B200: 333 of 1500 pages of 36 layers (1.57 GB read and
-// written) 257 us, 0.94 of the copy rate, after a plan of 11 us; 192 copies of 24 pages of 48 layers (302 MB written)
+// written) 257 us, 0.93 of the copy rate, after a plan of 11 us; 192 copies of 24 pages of 48 layers (302 MB written)
 // 69 us.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>

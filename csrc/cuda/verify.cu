@@ -21,9 +21,11 @@
 // is out, so that one or two are left, and only those are computed with the correctly rounded divisions and the full
 // exponential that the outcome is defined by: three divisions for each id take longer than reading it.  Sums are in fp32.
 //
-// Measured on one B200: 64 sequences with 0 to 4 drafts, 151936 ids, bf16: 21 us for 58 MB of logits and 20 us for the
-// draws (39 MB of noise), both bound by their instructions (14 a logit in the first); 24 sequences with a draft model's
-// probabilities in fp32 13 + 17 us; one sequence 15 us, a chain of dependent loads.
+// Measured on one B200: 64 sequences with 0 to 4 drafts, 151936 ids, bf16: 39 us in a CUDA graph, about half for the 52 MB
+// of logits (170 rows) and half for the draws (39 MB of noise).  Neither end is reached: the first launch runs 12
+// instructions a logit with 55 to 58% of the issue slots taken at 2.5 TB/s and 41% of the warps resident, the second 46% at
+// 1.7 TB/s and 27%, so that the latency of loads that too few warps cover bounds both.  24 sequences with a draft model's
+// probabilities in fp32 27 us; one sequence 14 us, a chain of dependent loads.
 #include <cfloat>
 
 #include <torch/extension.h>

@@ -246,7 +246,9 @@ def attn_shared_plan(block_tables, ctx_lens, group_offs, shared_lens, tokens: in
 def attn_shared(q, k_cache, v_cache, block_tables, plan: SharedPlan, out=None, scale: Optional[float] = None):
     """Attention of a step's query tokens q [T, Hq, D] (D = 64, 128 or 256) over the paged cache, for batches whose
     sequences come in groups that share a prefix's pages; query i of a sequence's nq sees its first
-    ctx - nq + i + 1 tokens.  Rows that see no token are zero.  ``plan``: from :func:`attn_shared_plan`."""
+    ctx - nq + i + 1 tokens.  Rows that see no token are zero.  Slots past a context may hold anything, but the V of a
+    query token has to be finite: the tokens before it give it weight 0, and 0 times NaN is NaN.  ``plan``: from
+    :func:`attn_shared_plan`."""
     if q.shape != plan.q_shape or k_cache.shape[1] != plan.kv_heads or block_tables.shape != plan.table_shape:
         raise ValueError("attn_shared: the plan was made for other shapes")
     if out is None:
