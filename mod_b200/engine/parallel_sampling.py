@@ -124,7 +124,7 @@ class ParallelSampler:
         T = len(ids)
         fb = ForwardBatch(input_ids=up(ids, torch.long), positions=up(np.concatenate(pos)),
                           slot_mapping=up(np.concatenate(slots)), block_tables=torch.from_numpy(bt).to(dev),
-                          ctx_lens=up(ctx), logits_idx=up(rows, torch.long),
+                          ctx_lens=up(ctx), logits_idx=torch.arange(T, device=dev) if len(rows) == T else up(rows, torch.long),
                           state_slots=up([s.state_slot for s in seqs], torch.long), is_decode=False, query_lens=qlens,
                           ctx_lens_host=ctx)
         if self.shared:  # one schedule for all layers of the step
